@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+from typing import NamedTuple
 
 import numpy as np
 
@@ -116,6 +117,8 @@ _sig("qeng_kv_append", _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp)
 _sig("qeng_attn_decode", _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _f32, _vp, _vp)
 _sig("qeng_attn_decode_ex", _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _f32, _f32, _i32, _vp, _vp)
 _sig("qeng_attn_decode_noalloc", _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _f32, _vp, _vp)
+_sig("qeng_kv_plan", _i32, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp)
+_sig("qeng_rope_append", _i32, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _vp, _f32, _vp, _i64, _vp)
 _sig("qeng_decoder_create", _i32, _vp, C.POINTER(ModelCfg), C.POINTER(_vp))
 _sig("qeng_decoder_free", _i32, _vp, _vp)
 _sig("qeng_decoder_load_matrix", _i32, _vp, _vp, _i32, _i32, _vp, _vp, _i64, _i64)
@@ -389,8 +392,74 @@ class Context:
                                                  _dev_ptr(lens), b, hq, scale, _dev_ptr(out), _cur_stream()))
         return out
 
+    # ---- serving -------------------------------------------------------------
+    def kv_plan_buffers(self, requests, capacity):
+        """Buffers for the results of kv_plan, to be used again from step to step (and by a captured one)."""
+        import torch
+        n, dev = requests, "cuda:%d" % self.device
+        ints = torch.empty(2 * n + 1 + 4 * capacity, dtype=torch.int32, device=dev)
+        starts, lens, slots, pos, seen, rows = ints.split([n + 1, n] + [capacity] * 4)
+        return KVPlan(starts, slots, pos, seen, rows, lens, torch.empty(2, dtype=torch.int64, device=dev))
+
+    def kv_plan(self, pool, lens, add, table, ring, ends, capacity, keep=None, out=None):
+        """Pages and slots for add[r] more tokens of every request, see qeng_kv_plan: the table and the ring are updated, the rest
+        comes back as a KVPlan.  `out`: a KVPlan to fill; its lens and ends may be the arguments themselves."""
+        import torch
+        n = lens.numel()
+        for t, ty in ((lens, torch.int32), (add, torch.int32), (table, torch.int32), (ring, torch.int32), (ends, torch.int64)):
+            assert t.is_cuda and t.dtype == ty and t.is_contiguous()
+        assert add.numel() == n and ends.numel() == 2 and table.dim() == 2 and table.shape[0] >= n
+        assert keep is None or (keep.is_cuda and keep.dtype == torch.int32 and keep.is_contiguous() and keep.numel() == n)
+        if out is None:
+            out = self.kv_plan_buffers(n, capacity)
+        assert out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
+        rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), table.shape[1],
+                               ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
+                               out.slots.data_ptr(), out.pos.data_ptr(), out.seen.data_ptr(), out.rows.data_ptr(), capacity, _cur_stream())
+        if rc:
+            self.check(rc)
+        return out
+
+    def rope_append(self, pool, qkv, pos, slots, base, q_gain=None, k_gain=None, eps=1e-5, out=None):
+        """Rows of q|k|v [T, (Hq + 2 Hkv) * 128] (float32, float16 or bfloat16; rows may be strided): optional RMS norm of the q and k
+        heads, rotation, k and v into the pool at `slots`; returns q as float16 [T, Hq, 128].  Rows with a negative slot are left alone
+        (those of a new result are then not initialised)."""
+        import torch
+        dt = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[qkv.dtype]
+        t, width = qkv.shape
+        hq = width // pool.hd - 2 * pool.kv_heads
+        assert qkv.is_cuda and qkv.stride(1) == 1 and width % pool.hd == 0
+        assert pos.dtype == slots.dtype == torch.int32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == slots.numel() == t
+        if out is None:
+            out = qkv.new_empty((t, hq, pool.hd), dtype=torch.float16)
+        assert out.dtype == torch.float16 and out.shape == (t, hq, pool.hd) and out.stride(2) == 1 and out.stride(1) == pool.hd
+        rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), dt, t, qkv.stride(0) if t > 1 else width, hq,
+                                   None if q_gain is None else _gain(q_gain), None if k_gain is None else _gain(k_gain), eps, pos.data_ptr(),
+                                   slots.data_ptr(), base, out.data_ptr(), out.stride(0) if t > 1 else hq * pool.hd, _cur_stream())
+        if rc:
+            self.check(rc)
+        return out
+
     def decoder(self, **kw):
         return Decoder(self, **kw)
+
+
+def _gain(t):
+    import torch
+    assert t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == 128
+    return t.data_ptr()
+
+
+class KVPlan(NamedTuple):
+    """What kv_plan works out: tokens of a request are starts[r] .. starts[r + 1] - 1; per token its slot, position, number of keys
+    attended and request; lengths and ring counters afterwards."""
+    starts: object
+    slots: object
+    pos: object
+    seen: object
+    rows: object
+    lens: object
+    ends: object
 
 
 class Weight:
@@ -443,7 +512,8 @@ class KVPool:
         self.ctx, self.h, self.pages, self.kv_heads, self.hd = ctx, h, pages, kv_heads, hd
 
     def tensor(self):
-        """The pool's storage as a torch f16 view [pages, kv_heads, 2, 16, hd]."""
+        """The pool's storage as a torch f16 view [pages, kv_heads, 2, 16, hd].  The pool stays while a view of it does, unless it is
+        freed by hand."""
         import torch
         n = self.pages * self.kv_heads * 2 * 16 * self.hd
         ptr = _lib.qeng_kv_pool_data(self.h)
@@ -451,6 +521,7 @@ class KVPool:
 
         class _Holder:
             __cuda_array_interface__ = iface
+            pool = self
         return torch.as_tensor(_Holder(), device="cuda:%d" % self.ctx.device).view(self.pages, self.kv_heads, 2, 16, self.hd)
 
     def free(self):

@@ -267,6 +267,36 @@ int32_t qeng_attn_decode_noalloc(qeng_ctx* ctx, const qeng_kv_pool* pool, const 
                                  const int32_t* page_table, int64_t max_pages, const int32_t* lens,
                                  int64_t B, int64_t Hq, float scale, float* out, void* stream);
 
+/* ---- serving: from request lengths to the attention of a batch (the reference's runtime serves one conversation at a
+ *      time and has no counterpart; the page size, the pool and the table are those of the calls above) ------------------
+ * Pages and slots for the next tokens of R requests, worked out on the device.  Request r has lens[r] tokens in its row of
+ * page_table (R rows of max_pages entries) and gets add[r] more; add[r] = 0 leaves it alone, add[r] < 0 ends it.  Free pages
+ * stand in ring[ring_size], a queue: ends[0] pages have been taken from it and ends[1] given to it so far (0 <= ends[1] -
+ * ends[0] <= ring_size; page number i is ring[i % ring_size]), so a new server fills ring with 0 .. pages - 1 and sets
+ * ends = {0, pages}.
+ *  - requests are served in order.  The first whose tokens exceed `capacity` together with those before it, or for whose pages the
+ *    ring has not enough, gets nothing, and no later one does; a request that would outgrow its table row, or whose length
+ *    makes no sense, gets nothing by itself (status 2).  New pages are written to the table.
+ *  - a request that ends gives its pages back, but for the first keep[r] (keep may be NULL: none), which it shares with others.
+ *    Pages given back are taken by later calls at the earliest.  Its length becomes 0, its row stays as it is.
+ *  - starts[R + 1]: the first token of every request, and their number; per token up to `capacity`: slots (16 * page + place in the
+ *    page), pos (its position), seen (pos + 1: the keys it attends), rows (its request).  Entries behind the last token are -1, 0, 0, -1.
+ *  - lens_out, ends_out: lengths and counters afterwards.  They may be lens and ends themselves.
+ * A page id outside the pool is reported (status 1), the slots in it are -1; so are counters that make no sense, or more pages given
+ * back than the ring has room for (status 6; then nothing is given back).  At most 8192 requests. */
+int32_t qeng_kv_plan(qeng_ctx* ctx, const qeng_kv_pool* pool, int64_t R, const int32_t* lens, const int32_t* add,
+                     const int32_t* keep, int32_t* page_table, int64_t max_pages, int32_t* ring, int64_t ring_size,
+                     const int64_t* ends, int32_t* lens_out, int64_t* ends_out, int32_t* starts, int32_t* slots,
+                     int32_t* pos, int32_t* seen, int32_t* rows, int64_t capacity, void* stream);
+/* T rows of q|k|v as a matmul leaves them ([T][Hq + 2 kv_heads][128] of x_dtype, ldx values from row to row) on their way to the
+ * attention: with q_gain and k_gain (f32[128], both or neither) every q and k head is RMS-normalised first; q and k are rotated as by
+ * qeng_rope at pos[t]; q goes to q_f16[t] (ldq values from row to row), k and v to place slots[t] of the pool, rounded to f16.  A row
+ * whose slot is negative is left alone: neither its q nor the pool is written.  A slot outside the pool is reported (status 1).  Slots of
+ * one call have to differ.  Rows, ldx * size, ldq * 2 and gains are 16-byte aligned. */
+int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int32_t x_dtype, int64_t T, int64_t ldx,
+                         int64_t Hq, const float* q_gain, const float* k_gain, float eps, const int32_t* pos,
+                         const int32_t* slots, float base, uint16_t* q_f16, int64_t ldq, void* stream);
+
 /* ---- the layer executor (the whole loop of decide/pipeline.md:51; what
  *      soma-kernel drives between SomaEvent::Prefill and SomaEvent::Answer,
  *      shell/src/worlds/soma_bridge.rs:244-277) -------------------------------- */
