@@ -138,6 +138,7 @@ extern "C" {
     pub fn qeng_attn_decode_noalloc(ctx: *mut qeng_ctx, pool: *const qeng_kv_pool, q_f16: *const u16, page_table: *const i32, max_pages: i64, lens: *const i32, B: i64, Hq: i64, scale: f32, out: *mut f32, stream: *mut c_void) -> i32;
     pub fn qeng_kv_plan(ctx: *mut qeng_ctx, pool: *const qeng_kv_pool, R: i64, lens: *const i32, add: *const i32, keep: *const i32, page_table: *mut i32, max_pages: i64, ring: *mut i32, ring_size: i64, ends: *const i64, lens_out: *mut i32, ends_out: *mut i64, starts: *mut i32, slots: *mut i32, pos: *mut i32, seen: *mut i32, rows: *mut i32, capacity: i64, stream: *mut c_void) -> i32;
     pub fn qeng_rope_append(ctx: *mut qeng_ctx, pool: *mut qeng_kv_pool, qkv: *const c_void, x_dtype: i32, T: i64, ldx: i64, Hq: i64, q_gain: *const f32, k_gain: *const f32, eps: f32, pos: *const i32, slots: *const i32, base: f32, q_f16: *mut u16, ldq: i64, stream: *mut c_void) -> i32;
+    pub fn qeng_attn_shared(ctx: *mut qeng_ctx, pool: *const qeng_kv_pool, q_f16: *const u16, ldq: i64, page_table: *const i32, max_pages: i64, table_rows: i64, rows: *const i32, lens: *const i32, T: i64, Hq: i64, group_first: *const i32, group_pages: *const i32, G: i64, scale: f32, softcap: f32, window: i32, out: *mut c_void, out_dtype: i32, ldo: i64, stream: *mut c_void) -> i32;
     pub fn qeng_decoder_create(ctx: *mut qeng_ctx, cfg: *const qeng_model_cfg, out: *mut *mut qeng_decoder) -> i32;
     pub fn qeng_decoder_free(ctx: *mut qeng_ctx, dec: *mut qeng_decoder) -> i32;
     pub fn qeng_decoder_load_matrix(ctx: *mut qeng_ctx, dec: *mut qeng_decoder, layer: i32, which: i32, q: *const u8, s: *const u16, N: i64, K: i64) -> i32;

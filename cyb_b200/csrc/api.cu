@@ -33,7 +33,7 @@ struct OutsideCapture {
 static void free_scratch(qeng_scratch* sc) {
   OutsideCapture outside;
   for (void* p : sc->kept) cudaFree(p);
-  for (qeng_buf* b : {&sc->planes, &sc->part, &sc->image, &sc->attn})
+  for (qeng_buf* b : {&sc->planes, &sc->part, &sc->image, &sc->shared, &sc->attn})
     if (b->ptr) cudaFree(b->ptr);
   delete sc;
 }

@@ -71,6 +71,7 @@ struct qeng_scratch {
   qeng_buf planes;    // activations as bf16 planes
   qeng_buf part;      // partial sums of tiles cut along K
   qeng_buf image;     // streaming matmul of more than 4 rows: activations quantised once, one image per K slice
+  qeng_buf shared;    // attention over shared pages: sums of what several CTAs found
   qeng_buf attn;      // decode attention: arrival counters (zero between calls), then the partials of the splits
   std::vector<void*> kept;  // captures: outgrown buffers that earlier nodes of the graph still use
 };

@@ -119,6 +119,7 @@ _sig("qeng_attn_decode_ex", _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _f3
 _sig("qeng_attn_decode_noalloc", _i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _f32, _vp, _vp)
 _sig("qeng_kv_plan", _i32, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp)
 _sig("qeng_rope_append", _i32, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _f32, _vp, _vp, _f32, _vp, _i64, _vp)
+_sig("qeng_attn_shared", _i32, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _f32, _f32, _i32, _vp, _i32, _i64, _vp)
 _sig("qeng_decoder_create", _i32, _vp, C.POINTER(ModelCfg), C.POINTER(_vp))
 _sig("qeng_decoder_free", _i32, _vp, _vp)
 _sig("qeng_decoder_load_matrix", _i32, _vp, _vp, _i32, _i32, _vp, _vp, _i64, _i64)
@@ -436,6 +437,30 @@ class Context:
         rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), dt, t, qkv.stride(0) if t > 1 else width, hq,
                                    None if q_gain is None else _gain(q_gain), None if k_gain is None else _gain(k_gain), eps, pos.data_ptr(),
                                    slots.data_ptr(), base, out.data_ptr(), out.stride(0) if t > 1 else hq * pool.hd, _cur_stream())
+        if rc:
+            self.check(rc)
+        return out
+
+    def attn_shared(self, pool, q, table, lens, group_first, group_pages, rows=None, scale=None, softcap=0.0, window=0, out=None, dtype=None):
+        """Attention of rows q [T, Hq, 128] (float16) over lens[t] tokens of table row rows[t] (None: t), where the rows
+        group_first[g] .. group_first[g + 1] - 1 share their first group_pages[g] pages; see qeng_attn_shared.  The result is `out`, or new, of
+        `dtype` (float32, float16 or bfloat16; None: float32); rows in no group, or of table row -1, are left alone (those of a new result
+        are then not initialised)."""
+        import torch
+        t, hq, hd = q.shape
+        assert q.dtype == torch.float16 and q.stride(2) == 1 and q.stride(1) == hd
+        for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
+            assert x.is_cuda and x.dtype == torch.int32 and x.is_contiguous()
+        g = group_pages.numel()
+        assert lens.numel() == t and group_first.numel() == g + 1 and table.dim() == 2 and (rows is None or rows.numel() == t)
+        if out is None:
+            out = q.new_empty((t, hq, hd), dtype=dtype or torch.float32)
+        assert out.shape == q.shape and dtype in (None, out.dtype) and out.stride(2) == 1 and out.stride(1) == hd
+        width = hq * hd
+        rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), q.stride(0) if t > 1 else width, table.data_ptr(), table.shape[1], table.shape[0],
+                                   None if rows is None else rows.data_ptr(), lens.data_ptr(), t, hq, group_first.data_ptr(), group_pages.data_ptr(), g,
+                                   float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(),
+                                   {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[out.dtype], out.stride(0) if t > 1 else width, _cur_stream())
         if rc:
             self.check(rc)
         return out

@@ -296,6 +296,23 @@ int32_t qeng_kv_plan(qeng_ctx* ctx, const qeng_kv_pool* pool, int64_t R, const i
 int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int32_t x_dtype, int64_t T, int64_t ldx,
                          int64_t Hq, const float* q_gain, const float* k_gain, float eps, const int32_t* pos,
                          const int32_t* slots, float base, uint16_t* q_f16, int64_t ldq, void* stream);
+/* out[t] = softmax(q[t] K^T * scale) V of every query head over the first lens[t] tokens of row rows[t] of page_table, for T rows
+ * in G groups.  Group g is rows group_first[g] .. group_first[g + 1] - 1 (group_first ascends, G + 1 entries); their table rows begin
+ * with the same group_pages[g] pages, which are read once for all of them (as the first row of the group lists them).  So a batch
+ * behind one prompt is a group whose pages are the prompt's, a prompt's own tokens are a group that shares all its pages (rows[t] the
+ * request, lens[t] = position + 1: what qeng_kv_plan writes), and a row without company is a group of one with no page shared.
+ *  - q_f16[t] and out[t] (f32, f16 or bf16) are [Hq][128], ldq and ldo values from row to row.  rows may be NULL: row t has table
+ *    row t.  A row in no group, or with rows[t] < 0, is left alone; one that attends nothing (lens[t] <= 0) gives zeros.
+ *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.
+ *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
+ *    results of the rows that attend it infinite or NaN, and of no other row.
+ * hd = 128, Hq / kv_heads <= 8, G <= 1024, T * Hq <= 2^21.  Bounds of groups that do not ascend, and rows outside the table, are
+ * reported (status 6; with such bounds nothing is written).  Needs working memory of the context. */
+int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, const uint16_t* q_f16, int64_t ldq,
+                         const int32_t* page_table, int64_t max_pages, int64_t table_rows, const int32_t* rows,
+                         const int32_t* lens, int64_t T, int64_t Hq, const int32_t* group_first,
+                         const int32_t* group_pages, int64_t G, float scale, float softcap, int32_t window, void* out,
+                         int32_t out_dtype, int64_t ldo, void* stream);
 
 /* ---- the layer executor (the whole loop of decide/pipeline.md:51; what
  *      soma-kernel drives between SomaEvent::Prefill and SomaEvent::Answer,
