@@ -1,15 +1,19 @@
 // Attention of rows (one query token each) over the paged f16 KV cache, where the rows of a group share their first pages: decode
 // batches behind one prompt, or the tokens of a prompt (a group whose rows share all pages and differ in length).
 //
-// Two kernels: attn_own_kernel reads the pages that a row has to itself, attn_join_kernel adds up what several CTAs found of a row.
-// Sums travel as (log2 of the largest weight m, sum l of 2^(x - m), sum of 2^(x - m) v): two of them add up after scaling by
-// 2^(m - max).
+// Three kernels: attn_tile_kernel works on the shared pages, every K and V read once for 256 rows of (token, head) and multiplied by
+// the 5th-generation tensor cores; attn_own_kernel reads the pages that a row has to itself and adds what the first found;
+// attn_join_kernel adds up what several CTAs found of a row.  Sums travel as (m, l = sum of 2^(x - m), sum of 2^(x - m) v), x a score in
+// the log2 domain: two of them add up after scaling by 2^(m - max).
 #include <cuda_bf16.h>
 #include <math.h>
 
 #include "attn_shared.h"
+#include "attn_tc.cuh"
 
 namespace {
+
+using namespace tc;
 
 constexpr int kHD = 128, kPage = 16;
 constexpr int kThreads = kOwnWarps * 32, kDepth = 2, kRing = kDepth * kOwnWarps;  // pages of a warp on their way
@@ -17,32 +21,9 @@ constexpr uint32_t kSlotBytes = 2 * kPage * kHD * 2;
 constexpr int kHDP = kHD + 4;  // row stride of the warps' sums in shared memory: no bank conflicts
 constexpr size_t kOwnSmem = kRing * kSlotBytes + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
-// The largest weight of a row is 2^kHigh: the smallest that a f16 number holds at full precision is then 2^-22 of it.
-constexpr float kHigh = 8.f;
+// The largest weight of a row is 2^kHigh and more: the smallest that a f16 number holds at full precision is then 2^-21 of it.
+constexpr float kHigh = 7.f;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count)); }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
-// Bounded wait: gives up (false) two seconds after the first failed attempt.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity) {
-  unsigned long long t0, t1;
-  asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t0));
-  do {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t1));
-  } while (t1 - t0 <= 2000000000ull);
-  return false;
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity); }
 // K and V of one (page, kv head): 32 rows as two halves of 64 dims, 128-byte swizzled
 __device__ __forceinline__ void page_g2s(uint32_t dst, const CUtensorMap* map, int row, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst), "l"(map), "r"(0),
@@ -65,10 +46,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // address of 16-byte chunk c (0..15) of row r (16..31: V) of a page
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)((c >> 3) * 4096 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -85,13 +62,31 @@ __device__ __forceinline__ void store4(const qeng_shared_attn& p, int t, int hq,
   }
 }
 
+// eight of them
+__device__ __forceinline__ void store8(const qeng_shared_attn& p, int t, int hq, int d, const float (&v)[8]) {
+  if (p.out_dtype == QENG_F32) {
+    store4(p, t, hq, d, make_float4(v[0], v[1], v[2], v[3]));
+    store4(p, t, hq, d + 4, make_float4(v[4], v[5], v[6], v[7]));
+    return;
+  }
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    h[i] = p.out_dtype == QENG_F16 ? pack_h2(v[2 * i], v[2 * i + 1]) : *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + (size_t)t * p.ldo + (size_t)hq * kHD + d) = make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 // ---- groups, rows and their units -----------------------------------------------------------------------------------------
 struct Groups {
-  int first[kSharedGroups + 1], pages[kSharedGroups];
+  int *first, *pages, *tile;  // [G + 1] each, in shared memory; tile: double tiles before a group
+  __device__ Groups(int* at, int G) : first(at), pages(at + G + 1), tile(at + 2 * (G + 1)) {}
 };
+constexpr size_t groups_bytes(int64_t G) { return (size_t)(3 * (G + 1)) * sizeof(int); }
 
 // Reads the groups into shared memory; false in every thread where their bounds do not ascend within the call's rows.
-__device__ __forceinline__ bool read_groups(const qeng_shared_attn& p, Groups& g) {
+__device__ __forceinline__ bool read_groups(const qeng_shared_attn& p, const Groups& g) {
   bool bad = false;
   for (int i = threadIdx.x; i <= p.G; i += blockDim.x) {
     const int f = p.first[i];
@@ -102,7 +97,36 @@ __device__ __forceinline__ bool read_groups(const qeng_shared_attn& p, Groups& g
     }
     bad = bad || f < 0 || f > p.T;
   }
-  return !__syncthreads_or(bad);
+  if (__syncthreads_or(bad)) return false;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int sum = 0;
+    for (int i = lane; i - lane < p.G; i += 32) {
+      const int n = i < p.G && g.pages[i] > 0 ? (g.first[i + 1] - g.first[i] + 2 * p.tokens - 1) / (2 * p.tokens) : 0;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (i < p.G) g.tile[i] = sum + x - n;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) g.tile[p.G] = sum;
+  }
+  __syncthreads();
+  return true;
+}
+
+// last i in [0, n) with a[i] <= x (a ascends, a[0] <= x)
+__device__ __forceinline__ int find(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 struct Row {
@@ -116,13 +140,7 @@ __device__ __forceinline__ Row row_of(const qeng_shared_attn& p, const Groups& g
   r.table_row = -1;
   r.len = r.win0 = r.group = r.page0 = r.pages = 0;
   if (t < g.first[0] || t >= g.first[p.G]) return r;
-  int lo = 0, hi = p.G;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (g.first[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  r.group = lo;
+  r.group = find(g.first, p.G, t);
   const int row = p.rows ? p.rows[t] : t;
   if (row < 0) return r;
   if (row >= p.table_rows) {
@@ -132,7 +150,7 @@ __device__ __forceinline__ Row row_of(const qeng_shared_attn& p, const Groups& g
   r.table_row = row;
   r.len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage);
   r.win0 = p.window > 0 ? max(0, r.len - p.window) : 0;
-  r.page0 = r.win0 / kPage;
+  r.page0 = max(r.win0 / kPage, g.pages[r.group]);
   r.pages = max(0, (r.len + kPage - 1) / kPage - r.page0);
   return r;
 }
@@ -141,13 +159,602 @@ __device__ __forceinline__ int units_of(const Row& r) { return (r.pages + kOwnWa
 // first CTA of `n` whose share of `all` units holds unit x, the shares beginning at c all / n
 __device__ __forceinline__ int cta_of(long long x, long long all, int n) { return (int)(((x + 1) * n - 1) / all); }
 
+// Adds up to 32 sums of one (row, head) to a running (M, L, O): lane i has the i-th, if any; its (m, l) and the place of its 128 values.
+// The lanes' pairs are loaded together and so are the values, four dims a lane.
+__device__ __forceinline__ void add_sums(int lane, bool have, const float2* ml_at, const float* o_at, float& M, float& L, float4& O) {
+  const float2 ml = have ? *ml_at : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m = fmaxf(m, M);
+  // (m, l) = (-inf, NaN): scores of NaN alone; (-inf, 0): nothing attended, or scores of minus infinity alone
+  const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m), a = M == -INFINITY ? 0.f : exp2f(M - m);
+  float l = ml.x == -INFINITY ? ml.y : ml.y * f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  L = (M == -INFINITY ? L : L * a) + l;
+  M = m;
+  O.x *= a; O.y *= a; O.z *= a; O.w *= a;
+  unsigned with = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+  while (with != 0) {
+    float4 v[4];
+    float g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = with != 0 ? __ffs(with) - 1 : -1;
+      const float* const at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)o_at, max(k, 0)));
+      g[i] = __shfl_sync(0xffffffffu, f, max(k, 0));
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k >= 0) v[i] = reinterpret_cast<const float4*>(at)[lane];
+      else g[i] = 0.f;
+      with &= with - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      O.x = fmaf(v[i].x, g[i], O.x); O.y = fmaf(v[i].y, g[i], O.y); O.z = fmaf(v[i].z, g[i], O.z); O.w = fmaf(v[i].w, g[i], O.w);
+    }
+  }
+}
+
+// What attn_tile_kernel found of row t: query head hq, dims 4 lane and on.  False: nothing there (no shared pages, or nobody in the
+// double tile attends any).  `whole`: how many CTAs it comes from is one.
+__device__ __forceinline__ bool shared_blocks(const qeng_shared_attn& p, const Groups& g, const Row& r, int t, int h, int& tile, int& c0, int& c1) {
+  if (g.pages[r.group] == 0) return false;
+  tile = g.tile[r.group] + (t - g.first[r.group]) / (2 * p.tokens);
+  const long long f0 = p.tile_first[tile], n = p.tile_first[tile + 1] - f0, all = (long long)p.tile_first[g.tile[p.G]] * p.Hkv;
+  if (n == 0) return false;
+  const long long x = f0 * p.Hkv + h * n;
+  c0 = cta_of(x, all, p.tile_ctas);
+  c1 = cta_of(x + n - 1, all, p.tile_ctas);
+  return true;
+}
+// Adds the pieces that CTAs c0 .. c1 of n have of something that all `all` units are divided for: piece i at `o` + 128 (stride (2 c + begins) + row)
+__device__ __forceinline__ void add_pieces(int lane, int c0, int c1, long long all, int n, const float* o, const float* ml, int stride, int row, float& M, float& L,
+                                           float4& O) {
+  for (int c = c0 + lane; c - lane <= c1; c += 32) {
+    const bool have = c <= c1 && all * c / n < all * (c + 1) / n;  // a CTA may have nothing
+    const size_t at = (size_t)(2 * c + (c == c0 ? 1 : 0)) * stride + row;  // the first CTA ends with it, the others begin with it
+    add_sums(lane, have, reinterpret_cast<const float2*>(ml) + at, o + at * kHD, M, L, O);
+  }
+}
+
+// ---- shared pages -------------------------------------------------------------------------------------------------------------
+// A double tile is two tiles of 128 MMA rows, each of `tokens` tokens x the query heads of a kv head, against the same keys, 128 (eight
+// pages) at a time.  Queries, K and V lie in shared memory, the scores S and the outputs O in tensor memory (256 columns a tile); the
+// weights P take the place of the scores, as one f16 number or two (f32 results).  Warps 0-3 and 4-7 are the softmax of the two tiles, a
+// lane a row; 8 issues the MMAs, 9 the copies, 10 and 11 look for values that are not finite.  The MMAs of one tile run beside the
+// softmax of the other.  O is rescaled only when a row's maximum has grown by more than 2^kGrow since it was last.
+//
+// K and V tiles: [2 halves of 64 dims][128 keys][128 bytes], 128-byte swizzled; K is a K-major operand of 128 columns, V an MN-major one.
+constexpr int kRows = 128, kKeys = 128;
+constexpr uint32_t kTileBytes = kRows * kHD * 2, kHalf = kTileBytes / 2;
+constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + 1, kCheckWarp = kLoadWarp + 1, kCheckWarps = 2;
+constexpr int kTileThreads = (kCheckWarp + kCheckWarps) * 32;
+constexpr size_t kTileSmem = 6 * kTileBytes + 1024;
+constexpr uint32_t kO = 128;   // columns of a tile: scores at 0
+constexpr float kGrow = 8.f;   // weights reach 2^(kHigh + kGrow), below the largest f16 number
+
+// Some blocks of a double tile.
+struct Piece {
+  int t0, ntok, tiles, h;
+  int keys;                // shared keys of the group
+  int page0, blocks;       // first page, blocks of 128 keys (none: no more pieces)
+  int kv0, kv1;            // keys that any row attends: [kv0, kv1)
+  int begin_max, end_min;  // keys that every row attends (which attends any)
+  int table_row, whole, slot;
+};
+// whether some row does not attend some key of block j
+__device__ __forceinline__ bool is_edge(const Piece& w, int j) {
+  const int key0 = w.page0 * kPage + j * kKeys;
+  return key0 < w.begin_max || key0 + kKeys > w.end_min;
+}
+
+// keys that the rows of a double tile attend among the shared ones, found by a warp
+__device__ __forceinline__ void span_of(const qeng_shared_attn& p, int lane, Piece& w) {
+  int kv0 = 0x7fffffff, kv1 = 0, begin_max = 0, end_min = 0x7fffffff, some = 0x7fffffff;
+  for (int i = lane; i < w.ntok; i += 32) {
+    const int t = w.t0 + i, row = p.rows ? p.rows[t] : t;
+    if (row < 0 || row >= p.table_rows) continue;
+    const int len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage), begin = p.window > 0 ? max(0, len - p.window) : 0, end = min(len, w.keys);
+    if (begin >= end) continue;
+    kv0 = min(kv0, begin);
+    kv1 = max(kv1, end);
+    begin_max = max(begin_max, begin);
+    end_min = min(end_min, end);
+    some = min(some, i);
+  }
+  w.kv0 = __reduce_min_sync(0xffffffffu, kv0);
+  w.kv1 = __reduce_max_sync(0xffffffffu, kv1);
+  w.begin_max = __reduce_max_sync(0xffffffffu, begin_max);
+  w.end_min = __reduce_min_sync(0xffffffffu, end_min);
+  some = __reduce_min_sync(0xffffffffu, some);
+  w.table_row = some == 0x7fffffff ? -1 : p.rows ? p.rows[w.t0 + some] : w.t0 + some;
+}
+__device__ __forceinline__ void rows_of_tile(const qeng_shared_attn& p, const Groups& g, int tile, Piece& w) {
+  const int k = find(g.tile, p.G, tile);  // the last group that begins here: the others are empty
+  w.t0 = g.first[k] + (tile - g.tile[k]) * 2 * p.tokens;
+  w.ntok = min(2 * p.tokens, g.first[k + 1] - w.t0);
+  w.tiles = w.ntok > p.tokens ? 2 : 1;
+  w.keys = (int)min((long long)g.pages[k] * kPage, 0x7fffffffll);
+}
+__device__ __forceinline__ int blocks_of(const Piece& w) { return w.kv1 > w.kv0 ? (w.kv1 - w.kv0 / kPage * kPage + kKeys - 1) / kKeys : 0; }
+
+struct TileShared {
+  int first[kSharedTiles + 1];  // blocks (of one kv head) before a double tile
+  Piece piece[2];
+  uint32_t bad[2][4];           // of a V tile: keys with a value that is not finite
+  int begun[2];                 // O of a tile holds sums before its first MMA
+  uint32_t tmem;
+  // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); scores and last outputs of a tile done, weights ready, V looked through
+  uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2], checked[2], drained;
+};
+
+template <bool kTwo>  // weights as two f16 numbers
+__global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ CUtensorMap qmap) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t qs = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = qs + 2 * kTileBytes;
+  __shared__ __align__(8) TileShared sh;
+  const Groups groups(reinterpret_cast<int*>(smem_raw + kTileSmem), p.G);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(sh.pfull + i), 1);
+      mbar_init(smem_u32(sh.pempty + i), kSoftWarps + 1 + kCheckWarps);
+      mbar_init(smem_u32(sh.sdone + i), 1);
+      mbar_init(smem_u32(sh.odone + i), 1);
+      mbar_init(smem_u32(sh.pready + i), kSoftWarps / 2);
+      mbar_init(smem_u32(sh.checked + i), kCheckWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(sh.full + i), 1);
+      mbar_init(smem_u32(sh.empty + i), i & 1 ? 1 + kCheckWarps : 1);
+    }
+    mbar_init(smem_u32(&sh.qfull), 1);
+    mbar_init(smem_u32(&sh.qempty), 1);
+    mbar_init(smem_u32(&sh.drained), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (!read_groups(p, groups)) {  // (attn_own_kernel reports it)
+    return;
+  }
+  const int ntiles = groups.tile[p.G];
+  for (int s = warp; s < ntiles; s += kTileThreads / 32) {
+    Piece w;
+    rows_of_tile(p, groups, s, w);
+    span_of(p, lane, w);
+    if (lane == 0) sh.first[s + 1] = blocks_of(w);
+  }
+  if (tid == 0) sh.first[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    int sum = 0;
+    for (int i = lane; i - lane < ntiles; i += 32) {
+      int x = i < ntiles ? sh.first[i + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (i < ntiles) sh.first[i + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+  } else if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&sh.tmem));
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (cta == 0)
+    for (int s = tid; s <= ntiles; s += kTileThreads) p.tile_first[s] = sh.first[s];
+  const uint32_t tmem = sh.tmem;
+  const long long all = (long long)sh.first[ntiles] * p.Hkv, u0 = all * cta / gridDim.x, u1 = all * (cta + 1) / gridDim.x;
+  bool failed = false;
+
+  // what a warp of another role does for the next piece's description; false: no more
+  int npiece = 0;
+  const auto next_piece = [&](Piece& w) {
+    const int e = npiece & 1;
+    if (!wait_warp(smem_u32(sh.pfull + e), (uint32_t)(npiece >> 1) & 1u)) {
+      failed = true;
+      return false;
+    }
+    w = sh.piece[e];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(sh.pempty + e));
+    ++npiece;
+    return w.blocks > 0;
+  };
+
+  if (warp == kLoadWarp) {
+    // ===== pieces and copies ============================================================================================
+    int n = 0, b = 0;  // pieces, blocks so far
+    long long u = u0;
+    int s = u < u1 ? find(sh.first, ntiles, (int)(u / p.Hkv)) : 0;
+    for (;;) {
+      Piece w;
+      w.blocks = 0;
+      int left = 0;  // blocks of the double tile and head from here on
+      if (u < u1) {
+        while ((long long)sh.first[s + 1] * p.Hkv <= u) ++s;
+        rows_of_tile(p, groups, s, w);
+        span_of(p, lane, w);
+        const int nb = sh.first[s + 1] - sh.first[s];
+        const long long at = u - (long long)sh.first[s] * p.Hkv;
+        w.h = (int)(at / nb);
+        const int k0 = (int)(at - (long long)w.h * nb);
+        left = nb - k0;
+        w.blocks = (int)min((long long)left, u1 - u);
+        w.page0 = w.kv0 / kPage + k0 * (kKeys / kPage);
+        w.whole = w.blocks == nb;
+        w.slot = 2 * cta + (k0 == 0 ? 1 : 0);
+      }
+      if (!wait_warp(smem_u32(sh.pempty + (n & 1)), ((uint32_t)(n >> 1) & 1u) ^ 1u)) { failed = true; break; }
+      if (lane == 0) {
+        sh.piece[n & 1] = w;
+        mbar_arrive(smem_u32(sh.pfull + (n & 1)));
+      }
+      __syncwarp();
+      if (w.blocks == 0) break;
+      const int last_page = (w.kv1 - 1) / kPage;
+      const int32_t* const ids = p.table + (size_t)w.table_row * p.max_pages;
+      // lanes 2 i and 2 i + 1 copy the two halves of page i of the block
+      const int pg = lane >> 1, half = lane & 1;
+      int id = lane < 16 && w.page0 + pg <= last_page ? ids[w.page0 + pg] : 0;
+      for (int j = 0; j < w.blocks && !failed; ++j, ++b) {
+        const int here = w.page0 + j * 8, pages = min(8, last_page - here + 1);
+        int row = id;
+        if ((unsigned)row >= (unsigned)p.pool_pages) {  // malformed page table: record it, read a page that exists
+          atomicExch(p.status, 1);
+          row = 0;
+        }
+        if (lane < 16 && j + 1 < w.blocks && here + 8 + pg <= last_page) id = ids[here + 8 + pg];
+        row = (row * p.Hkv + w.h) * 32;
+        for (int kv = 0; kv < 2; ++kv) {
+          const int slot = 2 * (b & 1) + kv;
+          const uint32_t bar = smem_u32(sh.full + slot);
+          if (!wait_warp(smem_u32(sh.empty + slot), ((uint32_t)(b >> 1) & 1u) ^ 1u)) { failed = true; break; }
+          if (lane == 0) mbar_expect_tx(bar, (uint32_t)pages * 4096u);
+          __syncwarp();
+          if (lane < 2 * pages)
+            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                             ring + (uint32_t)slot * kTileBytes + (uint32_t)half * kHalf + (uint32_t)pg * 2048u),
+                         "l"(&kvmap), "r"(0), "r"(row + 16 * kv), "r"(half), "r"(bar)
+                         : "memory");
+        }
+        if (j == 0 && !failed) {  // queries: half a tile at a time
+          if (!wait_warp(smem_u32(&sh.qempty), ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
+          if (lane == 0) mbar_expect_tx(smem_u32(&sh.qfull), (uint32_t)(w.tiles * 2 * 128 * p.grp * p.tokens));
+          __syncwarp();
+          if (lane < 2 * w.tiles)
+            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                             qs + (uint32_t)(lane >> 1) * kTileBytes + (uint32_t)half * kHalf),
+                         "l"(&qmap), "r"(64 * half), "r"(w.h * p.grp), "r"(w.t0 + (lane >> 1) * p.tokens), "r"(smem_u32(&sh.qfull))
+                         : "memory");
+        }
+      }
+      if (failed) break;
+      u += w.blocks;
+      ++n;
+    }
+  } else if (warp == kMmaWarp) {
+    // ===== MMA issue ====================================================================================================
+    // f16 x f16 -> f32, M = N = 128; B of S K-major, of O MN-major
+    constexpr uint32_t kIdescS = (1u << 4) | (16u << 17) | (8u << 24), kIdescO = kIdescS | (1u << 16);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, qs, 0), r0 = __shfl_sync(0xffffffffu, ring, 0);
+    int b = 0;                         // blocks so far
+    uint32_t turn[2] = {0, 0}, edges[2] = {0, 0};  // blocks of a tile; edges among the even and odd V tiles
+    const bool leader = elect_one();
+    const int who = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
+    Piece w;
+    while (next_piece(w)) {
+      bool lost = false;
+      if (leader) {
+        const auto scores = [&](int x, int blk) {
+          const uint64_t a = make_desc(q0 + (uint32_t)x * kTileBytes, 16, 1024), k = make_desc(r0 + (uint32_t)(2 * (blk & 1)) * kTileBytes, 16, 1024);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t at = (uint32_t)(i >> 2) * (kHalf >> 4) + (uint32_t)(i & 3) * 2u;
+            umma_ss(tm + (uint32_t)x * 256u, a + at, k + at, kIdescS, i > 0);
+          }
+          umma_commit(smem_u32(sh.sdone + x));
+        };
+        const auto full = [&](int kv, int blk) { return mbar_wait(smem_u32(sh.full + 2 * (blk & 1) + kv), (uint32_t)(blk >> 1) & 1u); };
+        lost = !mbar_wait(smem_u32(&sh.qfull), (uint32_t)(npiece - 1) & 1u) || !full(0, b);
+        if (!lost) {
+          fence_after();
+          for (int x = 0; x < w.tiles; ++x) scores(x, b);
+          umma_commit(smem_u32(sh.empty + 2 * (b & 1)));
+          if (w.blocks == 1) umma_commit(smem_u32(&sh.qempty));
+        }
+        for (int j = 0; j < w.blocks && !lost; ++j) {
+          const int blk = b + j, steps = min(8, (w.kv1 - (w.page0 + 8 * j) * kPage + kPage - 1) / kPage);
+          const bool edge = is_edge(w, j), more = j + 1 < w.blocks;
+          for (int x = 0; x < w.tiles; ++x) {
+            if (!mbar_wait(smem_u32(sh.pready + x), turn[x] & 1u)) { lost = true; break; }
+            ++turn[x];
+            if (x == 0) {
+              if (!full(1, blk)) { lost = true; break; }
+              if (edge && !mbar_wait(smem_u32(sh.checked + (blk & 1)), edges[blk & 1] & 1u)) { lost = true; break; }
+              edges[blk & 1] += edge;
+            }
+            fence_after();
+            const uint32_t o = tm + (uint32_t)x * 256u + kO, a = tm + (uint32_t)x * 256u;
+            const uint64_t v = make_desc(r0 + (uint32_t)(2 * (blk & 1) + 1) * kTileBytes, kHalf, 1024);
+            uint32_t acc = j > 0 || *(volatile int*)&sh.begun[x];
+            for (int k = 0; k < steps; ++k) {
+              umma_ts(o, a + 8u * k, v + (uint32_t)k * (2048u >> 4), kIdescO, acc);
+              if (kTwo) umma_ts(o, a + 64u + 8u * k, v + (uint32_t)k * (2048u >> 4), kIdescO, 1u);
+              acc = 1u;
+            }
+            if (x + 1 == w.tiles) umma_commit(smem_u32(sh.empty + 2 * (blk & 1) + 1));
+            if (!more) {
+              umma_commit(smem_u32(sh.odone + x));
+              continue;
+            }
+            if (x == 0 && !full(0, blk + 1)) { lost = true; break; }
+            fence_after();
+            scores(x, blk + 1);
+            if (x + 1 == w.tiles) {
+              umma_commit(smem_u32(sh.empty + 2 * ((blk + 1) & 1)));
+              if (j + 2 == w.blocks) umma_commit(smem_u32(&sh.qempty));
+            }
+          }
+        }
+        if (lost) {  // what was issued still has to finish before tensor memory is freed
+          umma_commit(smem_u32(&sh.drained));
+          mbar_wait(smem_u32(&sh.drained), 0);
+        }
+      }
+      lost = __shfl_sync(0xffffffffu, (int)lost, who);
+      if (lost) { failed = true; break; }
+      b += w.blocks;
+    }
+  } else if (warp >= kCheckWarp) {
+    // ===== values that are not finite ===================================================================================
+    // Where the rows of a block attend different keys, a value that is not finite would reach rows that do not attend it (their weight
+    // is zero, but zero times infinity is NaN).  Such keys are cleared here, and their rows added by the softmax; keys that nobody
+    // attends, and what no copy wrote, are cleared, too.
+    int b = 0;
+    Piece w;
+    while (next_piece(w) && !failed) {
+      for (int j = 0; j < w.blocks && !failed; ++j, ++b) {
+        // every tile is waited for, and let go: a parity says nothing to those who have missed a turn
+        if (!wait_warp(smem_u32(sh.full + 2 * (b & 1) + 1), (uint32_t)(b >> 1) & 1u)) { failed = true; break; }
+        if (!is_edge(w, j)) {
+          if (lane == 0) mbar_arrive(smem_u32(sh.empty + 2 * (b & 1) + 1));
+          continue;
+        }
+        const int key0 = (w.page0 + 8 * j) * kPage;
+        const uint32_t v = ring + (uint32_t)(2 * (b & 1) + 1) * kTileBytes;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int r = (warp - kCheckWarp) * 64 + 32 * i + lane;
+          const bool used = key0 + r >= w.kv0 && key0 + r < w.kv1;
+          uint32_t worst = 0;  // largest magnitude bits of the halves: an exponent of all ones has 0x7c00 and more
+          if (used) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              uint4 y;
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n"
+                           : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                           : "r"(v + (uint32_t)(c >> 3) * kHalf + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4))
+                           : "memory");
+              worst = __vmaxu2(worst, __vmaxu2(__vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu), __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu)));
+            }
+          }
+          const bool bad = (worst & 0xffffu) >= 0x7c00u || (worst >> 16) >= 0x7c00u;
+          if (!used || bad) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};\n" ::"r"(v + (uint32_t)(c >> 3) * kHalf + (uint32_t)r * 128u + (uint32_t)((c & 7) << 4)), "r"(0u) : "memory");
+          }
+          const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) sh.bad[b & 1][(warp - kCheckWarp) * 2 + i] = mask;
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(sh.checked + (b & 1)));
+          mbar_arrive(smem_u32(sh.empty + 2 * (b & 1) + 1));
+        }
+      }
+    }
+  } else {
+    // ===== softmax: this lane's row of tile x ============================================================================
+    const int x = warp >> 2, row = (warp & 3) * 32 + lane, tok = row / p.grp;
+    const uint32_t mem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)x * 256u;
+    const float sc = p.softcap > 0.f ? 1.f : p.scale * kLog2e;
+    const float cap2 = 2.f * kLog2e * p.scale / p.softcap, cap = p.softcap * kLog2e;
+    int b = 0;
+    uint32_t turn = 0, ends = 0, edges[2] = {0, 0};
+    Piece w;
+    while (next_piece(w) && !failed) {
+      if (x >= w.tiles) {
+        for (int j = 0; j < w.blocks; ++j) edges[(b + j) & 1] += is_edge(w, j);
+        b += w.blocks;
+        continue;
+      }
+      const int i = x * p.tokens + tok, t = w.t0 + i, head = w.h * p.grp + row - tok * p.grp;
+      bool live = tok < p.tokens && i < w.ntok;
+      int len = 0;
+      if (live) {
+        const int r = p.rows ? p.rows[t] : t;
+        live = r >= 0 && r < p.table_rows;
+        if (live) len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage);
+      }
+      const int win0 = p.window > 0 ? max(0, len - p.window) : 0;
+      const bool some = live && win0 < min(len, w.keys);
+      // a row that attends none of these keys attends everything, to nobody's use
+      const int begin = some ? win0 : 0, end = some ? min(len, w.keys) : 0x7fffffff;
+      float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < w.blocks; ++j, ++b) {
+        const int key0 = (w.page0 + 8 * j) * kPage;
+        const bool edge = is_edge(w, j);
+        if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
+        fence_after();
+        float s[kKeys];
+        tmem_ld128(mem, reinterpret_cast<uint32_t*>(s));
+        if (p.softcap > 0.f) {
+          // tanh y = 1 - 2 / (e^2y + 1), its error 2^-23 of the cap
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k) s[k] = fmaf(-2.f * cap, __frcp_rn(ex2(s[k] * cap2) + 1.f), cap);
+        }
+        if (edge) {
+          const int e = end - key0, a = begin - key0;
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k)
+            if (k >= e || k < a) s[k] = -INFINITY;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        // the reference of the row's weights moves when its maximum has left it far behind
+        const bool moved = mx > m_run && (m_run == -INFINITY || (mx - m_run) * sc > kGrow);
+        const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
+        if (moved) m_run = mx;
+        l_run *= alpha;
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(mem + kO + 32 * c, o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(mem + kO + 32 * c, o);
+          }
+        }
+        const float off = m_run == -INFINITY ? 0.f : kHigh - m_run * sc;  // nothing attended yet: all weights are zero
+        float sum[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // 32 keys at a time
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
+            fma2(a0, a1, sc, off);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
+            hi[k] = pack_h2(a0, a1);
+            if (kTwo) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+              lo[k] = pack_h2(a0 - f.x, a1 - f.y);
+            }
+          }
+          tmem_st16(mem + 16 * c, hi);
+          if (kTwo) tmem_st16(mem + 64 + 16 * c, lo);
+        }
+        l_run += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+        st_wait();
+        bool zeroed = false;
+        if (edge) {
+          if (!wait_warp(smem_u32(sh.checked + (b & 1)), edges[b & 1] & 1u)) { failed = true; break; }
+          ++edges[b & 1];
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll 1
+            for (uint32_t mask = sh.bad[b & 1][q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
+              const int k = 32 * q + __ffs(mask) - 1, key = key0 + k;
+              if (j == 0 && !zeroed) {
+                uint32_t z[32];
+#pragma unroll
+                for (int d = 0; d < 32; ++d) z[d] = 0u;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) tmem_st32(mem + kO + 32 * c, z);
+                st_wait();
+                zeroed = true;
+              }
+              float weight = 0.f;
+#pragma unroll 1
+              for (int c = 0; c <= (kTwo ? 64 : 0); c += 64) {
+                const uint32_t y = tmem_ld1(mem + c + k / 2);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
+                weight += k & 1 ? f.y : f.x;
+              }
+              const bool on = key >= begin && key < end;
+              const int id = p.table[(size_t)w.table_row * p.max_pages + key / kPage];
+              const __half2* const val = reinterpret_cast<const __half2*>(
+                  p.pool + (((size_t)((unsigned)id < (unsigned)p.pool_pages ? id : 0) * p.Hkv + w.h) * 32 + 16 + key % kPage) * kHD);
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                tmem_ld32(mem + kO + 32 * c, o);
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                  const float2 f = __half22float2(val[16 * c + d]);
+                  if (on) {
+                    o[2 * d] = __float_as_uint(fmaf(weight, f.x, __uint_as_float(o[2 * d])));
+                    o[2 * d + 1] = __float_as_uint(fmaf(weight, f.y, __uint_as_float(o[2 * d + 1])));
+                  }
+                }
+                __syncwarp();
+                tmem_st32(mem + kO + 32 * c, o);
+              }
+              st_wait();
+            }
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (j == 0 && (warp & 3) == 0) *(volatile int*)&sh.begun[x] = zeroed;
+          mbar_arrive(smem_u32(sh.pready + x));
+        }
+        ++turn;
+      }
+      if (failed || !wait_warp(smem_u32(sh.odone + x), ends & 1u)) { failed = true; break; }
+      ++ends;
+      fence_after();
+      // Whole and all that the row attends: its result.  Otherwise what has to be added to others' sums.
+      const bool alone = max((len + kPage - 1) / kPage - max(win0 / kPage, w.keys / kPage), 0) == 0;
+      const bool result = w.whole && alone;
+      const float inv = 1.f / l_run;
+      const size_t at = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
+      if (live && !result) {
+        float* const ml = (w.whole ? p.row_ml : p.tile_ml) + 2 * at;
+        // rows that attend nothing here have no weight
+        *reinterpret_cast<float2*>(ml) = some ? make_float2(m_run == -INFINITY ? -INFINITY : m_run * sc - kHigh, l_run) : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld32(mem + kO + 32 * c, o);
+        if (!live) continue;
+        if (result) {
+#pragma unroll
+          for (int d = 0; d < 32; d += 8) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = len == 0 ? 0.f : __uint_as_float(o[d + k]) * inv;
+            store8(p, t, head, 32 * c + d, f);
+          }
+        } else if (some) {
+          float4* const dst = reinterpret_cast<float4*>((w.whole ? p.row_o : p.tile_o) + at * kHD + 32 * c);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) dst[d] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (failed && lane == 0) atomicExch(p.status, 4);
+  fence_before();
+  if (__syncthreads_or(failed)) grace();
+  if (warp == kMmaWarp) tmem_free(tmem);
+}
+
 // ---- a row's own pages ------------------------------------------------------------------------------------------------------
 // A warp looks after the pages it reads, two on their way.  The query heads of the kv head are the eight columns of every MMA,
 // S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
 __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const ring = smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u;
-  __shared__ Groups groups;
+  const Groups groups(reinterpret_cast<int*>(smem_raw + kOwnSmem), p.G);
   __shared__ __align__(8) uint64_t full[kRing];
   __shared__ long long before[kThreads + 1];  // units before the rows of a thread
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, cta = blockIdx.x;
@@ -397,9 +1004,21 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
         L += sm_l[w][hh] * f;
         O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
       }
+      M -= kHigh;
       if (whole) {
+        const int hq = h * p.grp + hh;
+        const size_t place = (size_t)t * p.Hq + hq;
+        int tile, c0, c1;
+        if (shared_blocks(p, groups, row, t, h, tile, c0, c1)) {
+          if (c0 != c1) {  // attn_join_kernel adds this to the others' sums
+            reinterpret_cast<float4*>(p.row_o + place * kHD)[lane] = O;
+            if (lane == 0) reinterpret_cast<float2*>(p.row_ml)[place] = make_float2(M, L);
+            continue;
+          }
+          add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
+        }
         const float inv = 1.f / L;
-        store4(p, t, h * p.grp + hh, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
+        store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
       } else {
         const size_t at2 = (size_t)(2 * cta + (begins ? 1 : 0)) * 8 + hh;
         reinterpret_cast<float4*>(p.cut_o + at2 * kHD)[lane] = O;
@@ -417,45 +1036,56 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 constexpr int kJoinWarps = 8;
 
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_shared_attn p) {
-  __shared__ Groups groups;
+  extern __shared__ int join_smem[];
+  const Groups groups(join_smem, p.G);
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (!read_groups(p, groups)) return;
   const Row row = row_of(p, groups, t);
   if (row.table_row < 0) return;
   const long long u = p.unit_first[t], all = p.unit_first[p.T] * p.Hkv, units = p.unit_first[t + 1] - u;
   for (int hq = warp; hq < p.Hq; hq += kJoinWarps) {
-    if (units == 0) {
-      store4(p, t, hq, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
-      continue;
-    }
     const int h = hq / p.grp, hh = hq - h * p.grp;
-    const long long x = u * p.Hkv + h * units;
-    const int c0 = cta_of(x, all, p.own_ctas), c1 = cta_of(x + units - 1, all, p.own_ctas);
-    if (c0 == c1) continue;
+    int tile = 0, c0 = 0, c1 = 0, d0 = 0, d1 = 0;  // CTAs that worked on the shared pages, and on the row's own
+    const bool shared = shared_blocks(p, groups, row, t, h, tile, c0, c1);
+    if (units > 0) {
+      const long long x = u * p.Hkv + h * units;
+      d0 = cta_of(x, all, p.own_ctas);
+      d1 = cta_of(x + units - 1, all, p.own_ctas);
+    }
+    if (units == 0 ? shared && c0 == c1 : d0 == d1 && !(shared && c0 != c1)) continue;  // written by whom had all of it
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    const auto add = [&](const float* o, float2 ml) {
-      if (ml.x == -INFINITY) {  // nothing attended, or scores of minus infinity alone: no weight
-        L += ml.y;
-        return;
-      }
-      const float m = fmaxf(M, ml.x), a = M == -INFINITY ? 0.f : exp2f(M - m), f = exp2f(ml.x - m);
-      const float4 v = reinterpret_cast<const float4*>(o)[lane];
-      M = m;
-      L = L * a + ml.y * f;
-      O.x = O.x * a + v.x * f; O.y = O.y * a + v.y * f; O.z = O.z * a + v.z * f; O.w = O.w * a + v.w * f;
-    };
-    for (int c = c0; c <= c1; ++c) {
-      if (all * c / p.own_ctas == all * (c + 1) / p.own_ctas) continue;  // no units
-      const size_t at = (size_t)(2 * c + (c == c0 ? 1 : 0)) * 8 + hh;  // the first CTA ends with the pair, the others begin with it
-      add(p.cut_o + at * kHD, reinterpret_cast<const float2*>(p.cut_ml)[at]);
+    if (units > 0 && d0 != d1) add_pieces(lane, d0, d1, all, p.own_ctas, p.cut_o, p.cut_ml, 8, hh, M, L, O);
+    if (shared && c0 != c1) {
+      const int i = (t - groups.first[row.group]) % (2 * p.tokens);
+      add_pieces(lane, c0, c1, (long long)p.tile_first[groups.tile[p.G]] * p.Hkv, p.tile_ctas, p.tile_o, p.tile_ml, 256, i / p.tokens * 128 + i % p.tokens * p.grp + hh, M, L, O);
     }
-    const float inv = 1.f / L;
+    // of the two at most one is whole
+    const size_t place = (size_t)t * p.Hq + hq;
+    if ((shared && c0 == c1) || (units > 0 && d0 == d1)) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
+    const float inv = row.len == 0 ? 0.f : 1.f / L;
     store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
   }
 }
 
 }  // namespace
+
+// tensor maps of half a page's K or V (16 rows of 64 dims) and of half the queries of a tile ([tokens][grp] rows of 64 dims)
+static int32_t tile_maps(qeng_ctx* ctx, const qeng_shared_attn& p, CUtensorMap* kv, CUtensorMap* q) {
+  auto enc = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(qeng_tensor_map_encoder());
+  const cuuint32_t es[3] = {1, 1, 1};
+  const cuuint64_t kdims[3] = {64, (cuuint64_t)p.pool_pages * p.Hkv * 32, 2}, kstrides[2] = {256, 128};
+  const cuuint32_t kbox[3] = {64, kPage, 1};
+  const cuuint64_t qdims[3] = {kHD, (cuuint64_t)p.Hq, (cuuint64_t)p.T}, qstrides[2] = {kHD * 2, (cuuint64_t)p.ldq * 2};
+  const cuuint32_t qbox[3] = {64, (cuuint32_t)p.grp, (cuuint32_t)p.tokens};
+  if (!enc ||
+      enc(kv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.pool, kdims, kstrides, kbox, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+      enc(q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(p.q), qdims, qstrides, qbox, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return qeng_fail(ctx, QENG_ERR_CUDA, "attn_shared: tensor maps rejected");
+  return QENG_OK;
+}
 
 extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, const uint16_t* q_f16, int64_t ldq, const int32_t* page_table, int64_t max_pages,
                                     int64_t table_rows, const int32_t* rows, const int32_t* lens, int64_t T, int64_t Hq, const int32_t* group_first,
@@ -463,13 +1093,17 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
                                     int64_t ldo, void* stream) {
   if (!ctx || !pool || !q_f16 || !page_table || !lens || !group_first || !group_pages || !out) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: null argument");
   if (T <= 0 || Hq <= 0 || max_pages <= 0 || table_rows <= 0 || G <= 0) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: T, Hq, G and the table's sizes must be positive");
-  if (!(softcap >= 0.f) || window < 0) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: softcap and window must not be negative");
+  if (!(scale >= 0.f) || !(softcap >= 0.f) || window < 0) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: scale, softcap and window must not be negative");
   if (out_dtype < QENG_F32 || out_dtype > QENG_BF16) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: unknown type %d", out_dtype);
   if (Hq % pool->kv_heads != 0 || Hq / pool->kv_heads > 8)
     return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: query heads per kv head must divide evenly and be <= 8");
   if (G > kSharedGroups || T * Hq > (1 << 21) || max_pages > (1 << 26) || table_rows > (1 << 30) || pool->pages * pool->kv_heads >= (1 << 26))
     return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: at most %d groups, 2^21 rows times heads, less than 2^26 pages times kv heads", kSharedGroups);
   if (!rows && table_rows < T) return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: a table of %lld rows for %lld without their rows", (long long)table_rows, (long long)T);
+  const int grp = (int)(Hq / pool->kv_heads), tokens = 128 / grp;
+  const int64_t tiles = (T + 2 * tokens - 1) / (2 * tokens) + (G < T ? G : T);  // at most
+  if (tiles > kSharedTiles || (max_pages / 8 + 2) * tiles > 0x7fffffff)
+    return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: rows / %d + groups exceed %d, or their pages 2^34", 2 * tokens, kSharedTiles);
   if (ldq < Hq * kHD || ldo < Hq * kHD) return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: rows of %lld and %lld values hold less than %lld heads", (long long)ldq, (long long)ldo, (long long)Hq);
   if (((reinterpret_cast<uintptr_t>(q_f16) | reinterpret_cast<uintptr_t>(out)) & 15) != 0 || ldq % 8 != 0 || ldo % (out_dtype == QENG_F32 ? 4 : 8) != 0)
     return qeng_fail(ctx, QENG_ERR_ALIGN, "attn_shared: rows of q and out must be 16-byte aligned");
@@ -478,31 +1112,47 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   static bool configured_on[64] = {};  // the opt-in shared-memory size is set per device
   bool& configured = configured_on[ctx->device & 63];
   if (!configured) {
-    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_own_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOwnSmem));
+    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_tile_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTileSmem + groups_bytes(kSharedGroups))));
+    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_tile_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTileSmem + groups_bytes(kSharedGroups))));
+    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_own_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kOwnSmem + groups_bytes(kSharedGroups))));
     configured = true;
   }
   qeng_shared_attn p;
   p.q = reinterpret_cast<const __half*>(q_f16); p.ldq = ldq; p.table = page_table; p.max_pages = max_pages; p.table_rows = table_rows;
   p.rows = rows; p.lens = lens; p.first = group_first; p.pages = group_pages; p.out = out; p.ldo = ldo; p.out_dtype = out_dtype; p.status = ctx->status;
-  p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)pool->kv_heads; p.grp = (int)(Hq / pool->kv_heads); p.G = (int)G; p.pool_pages = (int)pool->pages;
-  p.window = window; p.scale = scale; p.softcap = softcap;
+  p.pool = pool->data; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)pool->kv_heads; p.grp = grp; p.tokens = tokens; p.G = (int)G; p.pool_pages = (int)pool->pages;
+  p.window = window; p.softcap = softcap;
+  p.scale = scale > 0.f ? scale : 1e-30f;  // nothing, but a masked score (minus infinity) stays what it is
   p.own_ctas = 3 * ctx->sm_count;
-  CUtensorMap map;
+  p.tile_ctas = ctx->sm_count;
+  CUtensorMap map, tile_map, q_map;
   int32_t rc = qeng_kv_map(ctx, pool->data, pool->pages * pool->kv_heads * 32, &map);
   if (rc != QENG_OK) return rc;
-  qeng_scratch* sc = qeng_scratch_for(ctx, st);
-  const size_t units = ((size_t)T + 1) * 8, cut = (size_t)2 * p.own_ctas * 8;
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  rc = qeng_scratch_grow(ctx, sc, &sc->shared, up(units) + up(cut * kHD * 4) + up(cut * 8));
+  rc = tile_maps(ctx, p, &tile_map, &q_map);
   if (rc != QENG_OK) return rc;
-  unsigned char* at = static_cast<unsigned char*>(sc->shared.ptr);
-  p.unit_first = reinterpret_cast<long long*>(at);
-  p.cut_o = reinterpret_cast<float*>(at += up(units));
-  p.cut_ml = reinterpret_cast<float*>(at += up(cut * kHD * 4));
-  p.own_o = p.own_ml = nullptr;
-  attn_own_kernel<<<(unsigned)p.own_ctas, kThreads, kOwnSmem, st>>>(p, map);
+  qeng_scratch* sc = qeng_scratch_for(ctx, st);
+  // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml
+  const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_ctas * 8;
+  const size_t need[8] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8};
+  size_t at[9] = {0};
+  for (int i = 0; i < 8; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
+  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[8]);
+  if (rc != QENG_OK) return rc;
+  unsigned char* const mem = static_cast<unsigned char*>(sc->shared.ptr);
+  p.tile_first = reinterpret_cast<int*>(mem);
+  p.tile_o = reinterpret_cast<float*>(mem + at[1]);
+  p.tile_ml = reinterpret_cast<float*>(mem + at[2]);
+  p.row_o = reinterpret_cast<float*>(mem + at[3]);
+  p.row_ml = reinterpret_cast<float*>(mem + at[4]);
+  p.unit_first = reinterpret_cast<long long*>(mem + at[5]);
+  p.cut_o = reinterpret_cast<float*>(mem + at[6]);
+  p.cut_ml = reinterpret_cast<float*>(mem + at[7]);
+  if (out_dtype == QENG_F32) attn_tile_kernel<true><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
+  else attn_tile_kernel<false><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   QENG_LAUNCH_CHECK(ctx);
-  attn_join_kernel<<<(unsigned)T, kJoinWarps * 32, 0, st>>>(p);
+  attn_own_kernel<<<(unsigned)p.own_ctas, kThreads, kOwnSmem + groups_bytes(G), st>>>(p, map);
+  QENG_LAUNCH_CHECK(ctx);
+  attn_join_kernel<<<(unsigned)T, kJoinWarps * 32, groups_bytes(G), st>>>(p);
   QENG_LAUNCH_CHECK(ctx);
   return QENG_OK;
 }

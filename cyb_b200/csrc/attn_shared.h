@@ -5,6 +5,7 @@
 #include "attn_prefill.h"
 
 constexpr int kSharedGroups = 1024;  // groups of rows in a call
+constexpr int kSharedTiles = 4096;   // and double tiles of them
 constexpr int kOwnWarps = 4;         // of a CTA that reads rows' own pages, and pages of a unit of its work
 
 struct qeng_shared_attn {
@@ -13,14 +14,21 @@ struct qeng_shared_attn {
   const int32_t* rows;     // [T] table row (negative: not there), or null: t
   const int32_t* lens;     // [T] keys
   const int32_t *first, *pages;  // [G + 1] rows of the groups, [G] pages that the rows of a group share
+  __half* pool;
   void* out;
   int32_t* status;
   long long ldq, ldo, max_pages, table_rows;
-  int out_dtype, T, Hq, Hkv, grp, G, pool_pages, window, own_ctas;
+  int out_dtype, T, Hq, Hkv, grp, tokens, G, pool_pages, window, own_ctas, tile_ctas;  // tokens: of a tile, 128 / grp
   float scale, softcap;
-  // Working memory.  Units of a row: its own pages by fours, for every kv head; the CTAs of attn_own_kernel divide all units evenly
-  // (CTA c: [c W / n, (c + 1) W / n)), so that a CTA has whole (row, kv head) pairs but for its first and last.
-  long long* unit_first;   // [T + 1] units (of one kv head) before a row
-  float *own_o, *own_ml;   // pairs with shared pages, too: [T][Hq][128] sums of weighted values, [T][Hq][2] (log2 of the largest weight, sum)
-  float *cut_o, *cut_ml;   // pairs cut between CTAs: [2 own_ctas][8][128], [..][2]: of the pair a CTA begins with, of the one it ends with
+  // Working memory: sums that are not a row's whole result, each with (m, l): the sum is of 2^(x - m) v, l of 2^(x - m).
+  //
+  // The shared pages of a group are worked on by double tiles: 2 * tokens rows, one kv head, all keys that any of them attends, by blocks
+  // of 128.  The CTAs of attn_tile_kernel divide all blocks evenly (CTA c: [c W / n, (c + 1) W / n) in the order of double tiles, kv
+  // heads, keys), so that a CTA has whole ones but for the first and the last.  The pages that a row has to itself are divided the same way
+  // among the CTAs of attn_own_kernel, in units of four pages.
+  int* tile_first;             // [double tiles + 1] blocks (of one kv head) before a double tile
+  float *tile_o, *tile_ml;     // cut between CTAs: [2 tile_ctas][256][128], [..][2]: of what a CTA begins with, of what it ends with
+  float *row_o, *row_ml;       // [T][Hq][128], [..][2]: the shared part of a row that has pages to itself, whole; or, where that is cut, the row's own, whole
+  long long* unit_first;       // [T + 1] units (of one kv head) before a row
+  float *cut_o, *cut_ml;       // cut between CTAs: [2 own_ctas][8][128], [..][2]
 };

@@ -306,7 +306,7 @@ int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int
  *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.
  *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
  *    results of the rows that attend it infinite or NaN, and of no other row.
- * hd = 128, Hq / kv_heads <= 8, G <= 1024, T * Hq <= 2^21.  Bounds of groups that do not ascend, and rows outside the table, are
+ * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do not ascend, and rows outside the table, are
  * reported (status 6; with such bounds nothing is written).  Needs working memory of the context. */
 int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, const uint16_t* q_f16, int64_t ldq,
                          const int32_t* page_table, int64_t max_pages, int64_t table_rows, const int32_t* rows,

@@ -128,6 +128,15 @@ def test_sizes(ctx, pages, rows):
     check(ctx, [behind(pages, [(7 * i) % 50 for i in range(rows)])], 16, 4, "float16" if rows % 2 else "float32", seed=rows)
 
 
+@pytest.mark.parametrize("pages", [299, 300, 304, 410, 1000])
+@pytest.mark.parametrize("rows", [2, 150])
+def test_many_blocks(ctx, pages, rows):
+    """Several blocks and pieces of kv heads to a CTA, whose last block is whole or not."""
+    check(ctx, [behind(pages, [(7 * i) % 50 for i in range(rows)])], 16, 8, seed=rows)
+    check(ctx, [(pages, [pages * 16 - 30 * i for i in range(rows)])], 32, 8, "float16", seed=rows)
+    check(ctx, [behind(pages, [i % 3 for i in range(rows)]), (pages - 37, [(pages - 37) * 16] * 40)], 8, 8, "bfloat16", window=4000)
+
+
 def test_rows_that_end_inside_what_they_share(ctx):
     """Lengths of nothing, of one token, of page and stage borders, of all but one."""
     lens = [0, 1, 15, 16, 17, 127, 128, 129, 255, 256, 257, 300, 319, 320, 321, 400]
@@ -376,11 +385,11 @@ def test_refusals(ctx):
     pool = ctx.kv_pool(4, 2)
     x = torch.zeros(4096, dtype=torch.float32, device="cuda").data_ptr()
 
-    def call(q=x, ldq=4 * HD, max_pages=1, table_rows=8, rows=x, lens=x, T=2, hq=4, first=x, G=1, cap=0.0, window=0, out=x, dt=0, ldo=4 * HD):
-        return qeng._lib.qeng_attn_shared(ctx.h, pool.h, q, ldq, x, max_pages, table_rows, rows, lens, T, hq, first, x, G, 1.0, cap, window, out, dt, ldo, None)
+    def call(q=x, ldq=4 * HD, max_pages=1, table_rows=8, rows=x, lens=x, T=2, hq=4, first=x, G=1, cap=0.0, window=0, out=x, dt=0, ldo=4 * HD, scale=1.0):
+        return qeng._lib.qeng_attn_shared(ctx.h, pool.h, q, ldq, x, max_pages, table_rows, rows, lens, T, hq, first, x, G, scale, cap, window, out, dt, ldo, None)
     for kw, code in [(dict(q=None), -1), (dict(lens=None), -1), (dict(first=None), -1), (dict(out=None), -1), (dict(T=0), -1), (dict(hq=0), -1),
-                     (dict(max_pages=0), -1), (dict(table_rows=0), -1), (dict(G=0), -1), (dict(cap=-1.0), -1), (dict(cap=math.nan), -1), (dict(window=-1), -1),
-                     (dict(dt=3), -1), (dict(dt=-1), -1), (dict(hq=3), -2), (dict(hq=18, ldq=18 * HD, ldo=18 * HD), -2), (dict(G=1025), -2),
+                     (dict(max_pages=0), -1), (dict(table_rows=0), -1), (dict(G=0), -1), (dict(cap=-1.0), -1), (dict(cap=math.nan), -1), (dict(window=-1), -1), (dict(scale=-1.0), -1), (dict(scale=math.nan), -1),
+                     (dict(dt=3), -1), (dict(dt=-1), -1), (dict(hq=3), -2), (dict(hq=18, ldq=18 * HD, ldo=18 * HD), -2), (dict(G=1025), -2), (dict(T=1 << 17, G=1024, hq=16, ldq=16 * HD, ldo=16 * HD, table_rows=1 << 17), -2),
                      (dict(T=1 << 20), -2), (dict(max_pages=(1 << 26) + 1), -2), (dict(rows=None, table_rows=1), -2), (dict(ldq=4 * HD - 8), -2),
                      (dict(ldo=4 * HD - 8), -2), (dict(q=x + 8), -3), (dict(out=x + 8), -3), (dict(ldq=4 * HD + 4), -3), (dict(ldo=4 * HD + 2), -3),
                      (dict(ldo=4 * HD + 4, dt=2), -3)]:
