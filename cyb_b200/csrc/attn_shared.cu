@@ -20,6 +20,7 @@ constexpr int kThreads = kOwnWarps * 32, kDepth = 2, kRing = kDepth * kOwnWarps;
 constexpr uint32_t kSlotBytes = 2 * kPage * kHD * 2;
 constexpr int kHDP = kHD + 4;  // row stride of the warps' sums in shared memory: no bank conflicts
 constexpr size_t kOwnSmem = kRing * kSlotBytes + 1024;
+constexpr int kChunks = 512;     // of rows, whose units are counted together
 constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row is 2^kHigh and more: the smallest that a f16 number holds at full precision is then 2^-21 of it.
 constexpr float kHigh = 7.f;
@@ -135,20 +136,21 @@ struct Row {
   int page0, pages;          // its own pages: the first, how many
 };
 
+__device__ __forceinline__ int table_row_of(const qeng_shared_attn& p, int t) {
+  const int row = p.rows ? __ldg(p.rows + t) : t;
+  return row < p.table_rows ? row : -1;
+}
+__device__ __forceinline__ int len_of(const qeng_shared_attn& p, int t) { return (int)min((long long)max(__ldg(p.lens + t), 0), p.max_pages * kPage); }
+
 __device__ __forceinline__ Row row_of(const qeng_shared_attn& p, const Groups& g, int t) {
   Row r;
   r.table_row = -1;
   r.len = r.win0 = r.group = r.page0 = r.pages = 0;
   if (t < g.first[0] || t >= g.first[p.G]) return r;
   r.group = find(g.first, p.G, t);
-  const int row = p.rows ? p.rows[t] : t;
-  if (row < 0) return r;
-  if (row >= p.table_rows) {
-    atomicExch(p.status, 6);
-    return r;
-  }
-  r.table_row = row;
-  r.len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage);
+  r.table_row = table_row_of(p, t);
+  if (r.table_row < 0) return r;
+  r.len = len_of(p, t);
   r.win0 = p.window > 0 ? max(0, r.len - p.window) : 0;
   r.page0 = max(r.win0 / kPage, g.pages[r.group]);
   r.pages = max(0, (r.len + kPage - 1) / kPage - r.page0);
@@ -156,8 +158,11 @@ __device__ __forceinline__ Row row_of(const qeng_shared_attn& p, const Groups& g
 }
 __device__ __forceinline__ int units_of(const Row& r) { return (r.pages + kOwnWarps - 1) / kOwnWarps; }
 
-// first CTA of `n` whose share of `all` units holds unit x, the shares beginning at c all / n
-__device__ __forceinline__ int cta_of(long long x, long long all, int n) { return (int)(((x + 1) * n - 1) / all); }
+// The CTAs of a kernel divide its work evenly: CTA c has the units [c q, (c + 1) q) of `all`, q = share(all, n).
+__device__ __forceinline__ long long divided(long long x, long long q) {  // of numbers that are not negative; most fit 32 bits
+  return ((unsigned long long)(x | q) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)q) : x / q;
+}
+__device__ __forceinline__ long long share(long long all, int n) { return max(divided(all + n - 1, n), 1ll); }
 
 // Adds up to 32 sums of one (row, head) to a running (M, L, O): lane i has the i-th, if any; its (m, l) and the place of its 128 values.
 // The lanes' pairs are loaded together and so are the values, four dims a lane.
@@ -196,25 +201,22 @@ __device__ __forceinline__ void add_sums(int lane, bool have, const float2* ml_a
   }
 }
 
-// What attn_tile_kernel found of row t: query head hq, dims 4 lane and on.  False: nothing there (no shared pages, or nobody in the
-// double tile attends any).  `whole`: how many CTAs it comes from is one.
-__device__ __forceinline__ bool shared_blocks(const qeng_shared_attn& p, const Groups& g, const Row& r, int t, int h, int& tile, int& c0, int& c1) {
+// The CTAs of attn_tile_kernel that worked on the double tile of row t and kv head h, c0 to c1; false: none did (no shared pages, or
+// nobody in the double tile attends any).
+__device__ __forceinline__ bool shared_ctas(const qeng_shared_attn& p, const Groups& g, const Row& r, int t, int h, int& c0, int& c1) {
   if (g.pages[r.group] == 0) return false;
-  tile = g.tile[r.group] + (t - g.first[r.group]) / (2 * p.tokens);
-  const long long f0 = p.tile_first[tile], n = p.tile_first[tile + 1] - f0, all = (long long)p.tile_first[g.tile[p.G]] * p.Hkv;
+  const int tile = g.tile[r.group] + (t - g.first[r.group]) / (2 * p.tokens), f0 = p.tile_first[tile], n = p.tile_first[tile + 1] - f0;
   if (n == 0) return false;
-  const long long x = f0 * p.Hkv + h * n;
-  c0 = cta_of(x, all, p.tile_ctas);
-  c1 = cta_of(x + n - 1, all, p.tile_ctas);
+  const int q = (int)share((long long)p.tile_first[g.tile[p.G]] * p.Hkv, p.tile_ctas), x = f0 * p.Hkv + h * n;
+  c0 = x / q;
+  c1 = (x + n - 1) / q;
   return true;
 }
-// Adds the pieces that CTAs c0 .. c1 of n have of something that all `all` units are divided for: piece i at `o` + 128 (stride (2 c + begins) + row)
-__device__ __forceinline__ void add_pieces(int lane, int c0, int c1, long long all, int n, const float* o, const float* ml, int stride, int row, float& M, float& L,
-                                           float4& O) {
+// Adds the pieces of CTAs c0 to c1 of something cut between them, at `row` of `stride` rows for each piece.
+__device__ __forceinline__ void add_pieces(int lane, int c0, int c1, const float* o, const float* ml, int stride, int row, float& M, float& L, float4& O) {
   for (int c = c0 + lane; c - lane <= c1; c += 32) {
-    const bool have = c <= c1 && all * c / n < all * (c + 1) / n;  // a CTA may have nothing
     const size_t at = (size_t)(2 * c + (c == c0 ? 1 : 0)) * stride + row;  // the first CTA ends with it, the others begin with it
-    add_sums(lane, have, reinterpret_cast<const float2*>(ml) + at, o + at * kHD, M, L, O);
+    add_sums(lane, c <= c1, reinterpret_cast<const float2*>(ml) + at, o + at * kHD, M, L, O);
   }
 }
 
@@ -231,7 +233,8 @@ constexpr uint32_t kTileBytes = kRows * kHD * 2, kHalf = kTileBytes / 2;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + 1, kCheckWarp = kLoadWarp + 1, kCheckWarps = 2;
 constexpr int kTileThreads = (kCheckWarp + kCheckWarps) * 32;
 constexpr size_t kTileSmem = 6 * kTileBytes + 1024;
-constexpr uint32_t kO = 128;   // columns of a tile: scores at 0
+// Columns of a tile: scores at 0; the weights of 64 keys take the place of their scores, the second terms 32 columns behind the first.
+constexpr uint32_t kO = 128;
 constexpr float kGrow = 8.f;   // weights reach 2^(kHigh + kGrow), below the largest f16 number
 
 // Some blocks of a double tile.
@@ -253,10 +256,8 @@ __device__ __forceinline__ bool is_edge(const Piece& w, int j) {
 __device__ __forceinline__ void span_of(const qeng_shared_attn& p, int lane, Piece& w) {
   int kv0 = 0x7fffffff, kv1 = 0, begin_max = 0, end_min = 0x7fffffff, some = 0x7fffffff;
   for (int i = lane; i < w.ntok; i += 32) {
-    const int t = w.t0 + i, row = p.rows ? p.rows[t] : t;
-    if (row < 0 || row >= p.table_rows) continue;
-    const int len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage), begin = p.window > 0 ? max(0, len - p.window) : 0, end = min(len, w.keys);
-    if (begin >= end) continue;
+    const int t = w.t0 + i, len = len_of(p, t), begin = p.window > 0 ? max(0, len - p.window) : 0, end = min(len, w.keys);
+    if (table_row_of(p, t) < 0 || begin >= end) continue;
     kv0 = min(kv0, begin);
     kv1 = max(kv1, end);
     begin_max = max(begin_max, begin);
@@ -268,7 +269,7 @@ __device__ __forceinline__ void span_of(const qeng_shared_attn& p, int lane, Pie
   w.begin_max = __reduce_max_sync(0xffffffffu, begin_max);
   w.end_min = __reduce_min_sync(0xffffffffu, end_min);
   some = __reduce_min_sync(0xffffffffu, some);
-  w.table_row = some == 0x7fffffff ? -1 : p.rows ? p.rows[w.t0 + some] : w.t0 + some;
+  w.table_row = some == 0x7fffffff ? -1 : table_row_of(p, w.t0 + some);
 }
 __device__ __forceinline__ void rows_of_tile(const qeng_shared_attn& p, const Groups& g, int tile, Piece& w) {
   const int k = find(g.tile, p.G, tile);  // the last group that begins here: the others are empty
@@ -277,7 +278,7 @@ __device__ __forceinline__ void rows_of_tile(const qeng_shared_attn& p, const Gr
   w.tiles = w.ntok > p.tokens ? 2 : 1;
   w.keys = (int)min((long long)g.pages[k] * kPage, 0x7fffffffll);
 }
-__device__ __forceinline__ int blocks_of(const Piece& w) { return w.kv1 > w.kv0 ? (w.kv1 - w.kv0 / kPage * kPage + kKeys - 1) / kKeys : 0; }
+__device__ __forceinline__ int blocks_of(int kv0, int kv1) { return kv1 > kv0 ? (kv1 - kv0 / kPage * kPage + kKeys - 1) / kKeys : 0; }
 
 struct TileShared {
   int first[kSharedTiles + 1];  // blocks (of one kv head) before a double tile
@@ -288,6 +289,13 @@ struct TileShared {
   // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); scores and last outputs of a tile done, weights ready, V looked through
   uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2], checked[2], drained;
 };
+
+// cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
+__device__ __forceinline__ float capped(float x, float cap2, float cap) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(ex2(x * cap2) + 1.f));
+  return fmaf(-2.f * cap, y, cap);
+}
 
 template <bool kTwo>  // weights as two f16 numbers
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ CUtensorMap qmap) {
@@ -314,15 +322,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     mbar_init(smem_u32(&sh.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (!read_groups(p, groups)) {  // (attn_own_kernel reports it)
-    return;
-  }
+  if (tid == 0) p.tile_jobs[cta].rows = 0;
+  if (!read_groups(p, groups)) return;  // (attn_own_kernel reports it)
   const int ntiles = groups.tile[p.G];
-  for (int s = warp; s < ntiles; s += kTileThreads / 32) {
-    Piece w;
-    rows_of_tile(p, groups, s, w);
-    span_of(p, lane, w);
-    if (lane == 0) sh.first[s + 1] = blocks_of(w);
+  {  // keys that the double tiles attend, a thread a row; the ring is not in use yet
+    int* const kv0 = reinterpret_cast<int*>(smem_raw);
+    int* const kv1 = kv0 + ntiles;
+    for (int s = tid; s < ntiles; s += kTileThreads) {
+      kv0[s] = 0x7fffffff;
+      kv1[s] = 0;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int t = groups.first[0] + tid; t < groups.first[p.G]; t += kTileThreads) {
+      const int g = find(groups.first, p.G, t), len = len_of(p, t), begin = p.window > 0 ? max(0, len - p.window) : 0, end = min(len, groups.pages[g] * kPage);
+      if (table_row_of(p, t) >= 0 && begin < end) {
+        const int s = groups.tile[g] + (t - groups.first[g]) / (2 * p.tokens);
+        atomicMin(kv0 + s, begin);
+        atomicMax(kv1 + s, end);
+      }
+    }
+    __syncthreads();
+    for (int s = tid; s < ntiles; s += kTileThreads) sh.first[s + 1] = blocks_of(kv0[s], kv1[s]);
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // copies write there
   }
   if (tid == 0) sh.first[0] = 0;
   __syncthreads();
@@ -340,6 +362,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     }
   } else if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&sh.tmem));
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   }
   fence_before();
   __syncthreads();
@@ -347,7 +370,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
   if (cta == 0)
     for (int s = tid; s <= ntiles; s += kTileThreads) p.tile_first[s] = sh.first[s];
   const uint32_t tmem = sh.tmem;
-  const long long all = (long long)sh.first[ntiles] * p.Hkv, u0 = all * cta / gridDim.x, u1 = all * (cta + 1) / gridDim.x;
+  const int all = sh.first[ntiles] * p.Hkv, q = (int)share(all, gridDim.x), u0 = min(all, cta * q), u1 = min(all, u0 + q);
   bool failed = false;
 
   // what a warp of another role does for the next piece's description; false: no more
@@ -368,25 +391,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
   if (warp == kLoadWarp) {
     // ===== pieces and copies ============================================================================================
     int n = 0, b = 0;  // pieces, blocks so far
-    long long u = u0;
-    int s = u < u1 ? find(sh.first, ntiles, (int)(u / p.Hkv)) : 0;
+    int u = u0, s = u < u1 ? find(sh.first, ntiles, u / p.Hkv) : 0;
     for (;;) {
       Piece w;
       w.blocks = 0;
-      int left = 0;  // blocks of the double tile and head from here on
       if (u < u1) {
-        while ((long long)sh.first[s + 1] * p.Hkv <= u) ++s;
+        while (sh.first[s + 1] * p.Hkv <= u) ++s;
         rows_of_tile(p, groups, s, w);
         span_of(p, lane, w);
-        const int nb = sh.first[s + 1] - sh.first[s];
-        const long long at = u - (long long)sh.first[s] * p.Hkv;
-        w.h = (int)(at / nb);
-        const int k0 = (int)(at - (long long)w.h * nb);
-        left = nb - k0;
-        w.blocks = (int)min((long long)left, u1 - u);
+        const int nb = sh.first[s + 1] - sh.first[s], at = u - sh.first[s] * p.Hkv;
+        w.h = at / nb;
+        const int k0 = at - w.h * nb;
+        w.blocks = min(nb - k0, u1 - u);
         w.page0 = w.kv0 / kPage + k0 * (kKeys / kPage);
         w.whole = w.blocks == nb;
         w.slot = 2 * cta + (k0 == 0 ? 1 : 0);
+        if (k0 == 0 && !w.whole && lane == 0) {  // cut: attn_join_kernel adds the pieces
+          qeng_tile_job& job = p.tile_jobs[cta];
+          job.t0 = w.t0;
+          job.h = w.h;
+          job.last = (u + nb - 1) / q;
+          job.rows = w.ntok * p.grp;
+        }
       }
       if (!wait_warp(smem_u32(sh.pempty + (n & 1)), ((uint32_t)(n >> 1) & 1u) ^ 1u)) { failed = true; break; }
       if (lane == 0) {
@@ -482,8 +508,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
             const uint64_t v = make_desc(r0 + (uint32_t)(2 * (blk & 1) + 1) * kTileBytes, kHalf, 1024);
             uint32_t acc = j > 0 || *(volatile int*)&sh.begun[x];
             for (int k = 0; k < steps; ++k) {
-              umma_ts(o, a + 8u * k, v + (uint32_t)k * (2048u >> 4), kIdescO, acc);
-              if (kTwo) umma_ts(o, a + 64u + 8u * k, v + (uint32_t)k * (2048u >> 4), kIdescO, 1u);
+              const uint32_t w_at = a + 64u * (k >> 2) + 8u * (k & 3);
+              umma_ts(o, w_at, v + (uint32_t)k * (2048u >> 4), kIdescO, acc);
+              if (kTwo) umma_ts(o, w_at + 32u, v + (uint32_t)k * (2048u >> 4), kIdescO, 1u);
               acc = 1u;
             }
             if (x + 1 == w.tiles) umma_commit(smem_u32(sh.empty + 2 * (blk & 1) + 1));
@@ -578,9 +605,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       bool live = tok < p.tokens && i < w.ntok;
       int len = 0;
       if (live) {
-        const int r = p.rows ? p.rows[t] : t;
-        live = r >= 0 && r < p.table_rows;
-        if (live) len = (int)min((long long)max(p.lens[t], 0), p.max_pages * kPage);
+        live = table_row_of(p, t) >= 0;
+        if (live) len = len_of(p, t);
       }
       const int win0 = p.window > 0 ? max(0, len - p.window) : 0;
       const bool some = live && win0 < min(len, w.keys);
@@ -593,23 +619,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         const bool edge = is_edge(w, j);
         if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
         fence_after();
-        float s[kKeys];
-        tmem_ld128(mem, reinterpret_cast<uint32_t*>(s));
-        if (p.softcap > 0.f) {
-          // tanh y = 1 - 2 / (e^2y + 1), its error 2^-23 of the cap
+        // 64 keys at a time: the first half's scores are read twice, once for the maximum
+        float s[64];
+        const auto masked = [&](int half) {
+          if (!edge) return;
+          const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
 #pragma unroll
-          for (int k = 0; k < kKeys; ++k) s[k] = fmaf(-2.f * cap, __frcp_rn(ex2(s[k] * cap2) + 1.f), cap);
-        }
-        if (edge) {
-          const int e = end - key0, a = begin - key0;
-#pragma unroll
-          for (int k = 0; k < kKeys; ++k)
+          for (int k = 0; k < 64; ++k)
             if (k >= e || k < a) s[k] = -INFINITY;
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        };
+        float mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kKeys; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        for (int half = 0; half < 2; ++half) {
+          tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
+          masked(half);
+          float mx4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < 64; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
+          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        }
+        if (p.softcap > 0.f && mx != -INFINITY) mx = capped(mx, cap2, cap);
         // the reference of the row's weights moves when its maximum has left it far behind
         const bool moved = mx > m_run && (m_run == -INFINITY || (mx - m_run) * sc > kGrow);
         const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
@@ -630,23 +659,35 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // 32 keys at a time
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
-            fma2(a0, a1, sc, off);
-            a0 = ex2(a0);
-            a1 = ex2(a1);
-            add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
-            hi[k] = pack_h2(a0, a1);
-            if (kTwo) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              lo[k] = pack_h2(a0 - f.x, a1 - f.y);
-            }
+        for (int half = 1; half >= 0; --half) {
+          if (half == 0) {
+            tmem_ld64(mem, reinterpret_cast<uint32_t*>(s));
+            if (!(p.softcap > 0.f)) masked(0);
           }
-          tmem_st16(mem + 16 * c, hi);
-          if (kTwo) tmem_st16(mem + 64 + 16 * c, lo);
+          if (p.softcap > 0.f) {
+#pragma unroll
+            for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
+            masked(half);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // 32 keys at a time
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
+              fma2(a0, a1, sc, off);
+              a0 = ex2(a0);
+              a1 = ex2(a1);
+              add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
+              hi[k] = pack_h2(a0, a1);
+              if (kTwo) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                lo[k] = pack_h2(a0 - f.x, a1 - f.y);
+              }
+            }
+            tmem_st16(mem + 64 * half + 16 * c, hi);
+            if (kTwo) tmem_st16(mem + 64 * half + 32 + 16 * c, lo);
+          }
         }
         l_run += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         st_wait();
@@ -670,8 +711,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
               }
               float weight = 0.f;
 #pragma unroll 1
-              for (int c = 0; c <= (kTwo ? 64 : 0); c += 64) {
-                const uint32_t y = tmem_ld1(mem + c + k / 2);
+              for (int c = 0; c <= (kTwo ? 32 : 0); c += 32) {
+                const uint32_t y = tmem_ld1(mem + (k & 64) + c + (k & 63) / 2);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
                 weight += k & 1 ? f.y : f.x;
               }
@@ -711,10 +752,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       fence_after();
       // Whole and all that the row attends: its result.  Otherwise what has to be added to others' sums.
       const bool alone = max((len + kPage - 1) / kPage - max(win0 / kPage, w.keys / kPage), 0) == 0;
-      const bool result = w.whole && alone;
+      const bool result = w.whole && alone;  // (attn_own_kernel writes the zeros of a row that attends nothing)
       const float inv = 1.f / l_run;
       const size_t at = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
-      if (live && !result) {
+      if (live && !(w.whole && alone)) {
         float* const ml = (w.whole ? p.row_ml : p.tile_ml) + 2 * at;
         // rows that attend nothing here have no weight
         *reinterpret_cast<float2*>(ml) = some ? make_float2(m_run == -INFINITY ? -INFINITY : m_run * sc - kHigh, l_run) : make_float2(-INFINITY, 0.f);
@@ -724,16 +765,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         uint32_t o[32];
         __syncwarp();
         tmem_ld32(mem + kO + 32 * c, o);
-        if (!live) continue;
+        if (!some) continue;
         if (result) {
 #pragma unroll
           for (int d = 0; d < 32; d += 8) {
             float f[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = len == 0 ? 0.f : __uint_as_float(o[d + k]) * inv;
+            for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[d + k]) * inv;
             store8(p, t, head, 32 * c + d, f);
           }
-        } else if (some) {
+        } else {
           float4* const dst = reinterpret_cast<float4*>((w.whole ? p.row_o : p.tile_o) + at * kHD + 32 * c);
 #pragma unroll
           for (int d = 0; d < 8; ++d) dst[d] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
@@ -752,52 +793,78 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 // A warp looks after the pages it reads, two on their way.  The query heads of the kv head are the eight columns of every MMA,
 // S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
 __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const ring = smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u;
   const Groups groups(reinterpret_cast<int*>(smem_raw + kOwnSmem), p.G);
   __shared__ __align__(8) uint64_t full[kRing];
-  __shared__ long long before[kThreads + 1];  // units before the rows of a thread
+  __shared__ long long before[kChunks + 1];  // units before chunks of rows
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, cta = blockIdx.x;
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(full + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    p.own_jobs[cta].t = -1;
   }
   if (!read_groups(p, groups)) {
     if (cta == 0 && tid == 0) atomicExch(p.status, 6);
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     return;
   }
-  // units of all rows: a thread adds up neighbouring rows
-  const int per = (p.T + kThreads - 1) / kThreads;
-  {
-    long long n = 0;
-    for (int t = tid * per; t < min((tid + 1) * per, p.T); ++t) n += units_of(row_of(p, groups, t));
-    before[tid + 1] = n;
-    if (tid == 0) before[0] = 0;
-    __syncthreads();
-    if (warp == 0) {
-      long long sum = 0;
-      for (int i = 0; i < kOwnWarps; ++i) {
-        long long x = before[1 + i * 32 + lane];
+  // units of all rows, 32 rows to a warp at a time
+  const int per = 32 * ((p.T + 32 * kChunks - 1) / (32 * kChunks)), chunks = (p.T + per - 1) / per;
+#pragma unroll 4
+  for (int c = warp; c < chunks; c += kOwnWarps) {
+    int n = 0;  // (of 32 rows; of all rows of a chunk at most 2^16 * 2^24)
+    long long sum = 0;
+    for (int t = c * per + lane; t - lane < min((c + 1) * per, p.T); t += 32) {
+      n = t < p.T ? units_of(row_of(p, groups, t)) : 0;
+      sum += n;
+    }
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
-        }
-        before[1 + i * 32 + lane] = sum + x;
-        sum += __shfl_sync(0xffffffffu, x, 31);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) before[c + 1] = sum;
+  }
+  if (tid == 0) before[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    long long sum = 0;
+    for (int i = lane; i - lane < chunks; i += 32) {
+      long long x = i < chunks ? before[i + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
+      if (i < chunks) before[i + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
     }
-    __syncthreads();
   }
-  if (cta == 0) {  // for attn_join_kernel
-    long long n = before[tid];
-    for (int t = tid * per; t < min((tid + 1) * per, p.T); ++t) {
-      p.unit_first[t] = n;
-      n += units_of(row_of(p, groups, t));
+  __syncthreads();
+  // for attn_join_kernel, and rows that attend nothing: chunks in turn to the CTAs' warps
+  for (int c = cta + warp * (int)gridDim.x; c < chunks; c += kOwnWarps * (int)gridDim.x) {
+    long long sum = before[c];
+    for (int t0 = c * per; t0 < min((c + 1) * per, p.T); t0 += 32) {
+      const int t = t0 + lane;
+      Row r;
+      r.table_row = -1;
+      if (t < p.T) r = row_of(p, groups, t);
+      if (t < p.T && t >= groups.first[0] && t < groups.first[p.G] && p.rows && __ldg(p.rows + t) >= p.table_rows) atomicExch(p.status, 6);
+      const long long n = r.table_row >= 0 ? units_of(r) : 0;
+      long long x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (t < p.T) p.unit_first[t] = sum + x - n;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+      for (unsigned empty = __ballot_sync(0xffffffffu, r.table_row >= 0 && r.len == 0); empty != 0; empty &= empty - 1)
+        for (int hq = 0; hq < p.Hq; ++hq) store4(p, t0 + __ffs(empty) - 1, hq, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
     }
-    if (tid == 0) p.unit_first[p.T] = before[kThreads];
   }
-  const long long all = before[kThreads] * p.Hkv, u0 = all * cta / gridDim.x, u1 = all * (cta + 1) / gridDim.x;
+  const long long all = before[chunks] * p.Hkv, q = share(all, gridDim.x), u0 = min(all, cta * q), u1 = min(all, u0 + q);
+  if (cta == 0 && tid == 0) p.unit_first[p.T] = before[chunks];
+  bool waited = false;  // for attn_tile_kernel
 
   float (*const sm_o)[8][kHDP] = reinterpret_cast<float (*)[8][kHDP]>(ring);
   float (*const sm_m)[8] = reinterpret_cast<float (*)[8]>(ring + sizeof(float) * kOwnWarps * 8 * kHDP);
@@ -810,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
   bool failed = false;
   for (long long u = u0; u < u1;) {
     // the pair of unit u: its rows' thread, then the row among that thread's, 32 at a time
-    int lo = 0, hi = kThreads;
+    int lo = 0, hi = chunks;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (before[mid] * p.Hkv <= u) lo = mid;
@@ -837,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
       at += __shfl_sync(0xffffffffu, n, 31) * p.Hkv;
     }
     row = row_of(p, groups, t);
-    const int units = units_of(row), h = (int)((u - at) / units);
+    const int units = units_of(row), h = (int)divided(u - at, units);
     const long long pair0 = at + (long long)h * units;       // the pair's units: [pair0, pair0 + units)
     const long long end = min(u1, pair0 + units);
     const int first = row.page0 + (int)(u - pair0) * kOwnWarps, last = min(row.page0 + row.pages, row.page0 + (int)(end - pair0) * kOwnWarps);
@@ -991,6 +1058,17 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
     }
     __syncthreads();
     const bool whole = begins && ends;
+    if (!waited) asm volatile("griddepcontrol.wait;\n" ::: "memory");  // what attn_tile_kernel found is there
+    waited = true;
+    int c0 = 0, c1 = 0;
+    const bool shared = shared_ctas(p, groups, row, t, h, c0, c1);
+    if (begins && !ends && !(shared && c0 != c1) && tid == 0) {  // cut, and no tile's job: attn_join_kernel adds the pieces
+      qeng_own_job& job = p.own_jobs[cta];
+      job.t = t;
+      job.h = h;
+      job.last = (int)divided(pair0 + units - 1, q);
+      job.shared = shared;
+    }
     for (int hh = warp; hh < p.grp; hh += kOwnWarps) {
       float M = -INFINITY;
 #pragma unroll
@@ -1005,66 +1083,68 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
         O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
       }
       M -= kHigh;
-      if (whole) {
-        const int hq = h * p.grp + hh;
+      const int hq = h * p.grp + hh;
+      if (whole && !(shared && c0 != c1)) {
         const size_t place = (size_t)t * p.Hq + hq;
-        int tile, c0, c1;
-        if (shared_blocks(p, groups, row, t, h, tile, c0, c1)) {
-          if (c0 != c1) {  // attn_join_kernel adds this to the others' sums
-            reinterpret_cast<float4*>(p.row_o + place * kHD)[lane] = O;
-            if (lane == 0) reinterpret_cast<float2*>(p.row_ml)[place] = make_float2(M, L);
-            continue;
-          }
-          add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
-        }
+        if (shared) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
         const float inv = 1.f / L;
         store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
-      } else {
-        const size_t at2 = (size_t)(2 * cta + (begins ? 1 : 0)) * 8 + hh;
-        reinterpret_cast<float4*>(p.cut_o + at2 * kHD)[lane] = O;
-        if (lane == 0) reinterpret_cast<float2*>(p.cut_ml)[at2] = make_float2(M, L);
+      } else {  // whole: a tile's job adds it to the pieces of the shared pages
+        float* const o_at = whole ? p.row_o : p.cut_o;
+        float* const ml_at = whole ? p.row_ml : p.cut_ml;
+        const size_t place = whole ? (size_t)t * p.Hq + hq : (size_t)(2 * cta + (begins ? 1 : 0)) * 8 + hh;
+        reinterpret_cast<float4*>(o_at + place * kHD)[lane] = O;
+        if (lane == 0) reinterpret_cast<float2*>(ml_at)[place] = make_float2(M, L);
       }
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the ring is written by copies again
     __syncthreads();
     u = end;
   }
+  if (!waited) asm volatile("griddepcontrol.wait;\n" ::: "memory");  // attn_join_kernel waits for both by waiting for this one
   if (__syncthreads_or(failed) && tid == 0) atomicExch(p.status, 4);
 }
 
-// ---- what is left of a row: sums of several CTAs, or nothing to attend --------------------------------------------------------
-constexpr int kJoinWarps = 8;
+// ---- what was cut between CTAs: a CTA of attn_tile_kernel left a job for the double tile (and kv head) that it ends with, a CTA of
+// attn_own_kernel for its last (row, kv head).  A tile's job also takes its rows' own sums, cut or whole.
+constexpr int kJoinWarps = 8, kJoinParts = 16;  // CTAs to a tile's job
 
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_shared_attn p) {
-  extern __shared__ int join_smem[];
-  const Groups groups(join_smem, p.G);
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (!read_groups(p, groups)) return;
-  const Row row = row_of(p, groups, t);
-  if (row.table_row < 0) return;
-  const long long u = p.unit_first[t], all = p.unit_first[p.T] * p.Hkv, units = p.unit_first[t + 1] - u;
-  for (int hq = warp; hq < p.Hq; hq += kJoinWarps) {
-    const int h = hq / p.grp, hh = hq - h * p.grp;
-    int tile = 0, c0 = 0, c1 = 0, d0 = 0, d1 = 0;  // CTAs that worked on the shared pages, and on the row's own
-    const bool shared = shared_blocks(p, groups, row, t, h, tile, c0, c1);
-    if (units > 0) {
-      const long long x = u * p.Hkv + h * units;
-      d0 = cta_of(x, all, p.own_ctas);
-      d1 = cta_of(x + units - 1, all, p.own_ctas);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const long long all = p.unit_first[p.T] * p.Hkv, q = share(all, p.own_ctas);
+  if (blockIdx.x < p.tile_ctas * kJoinParts) {
+    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts;
+    const qeng_tile_job job = p.tile_jobs[cta];
+    for (int r = part * kJoinWarps + warp; r < job.rows; r += kJoinParts * kJoinWarps) {
+      const int i = r / p.grp, hh = r - i * p.grp, t = job.t0 + i, hq = job.h * p.grp + hh;
+      if (table_row_of(p, t) < 0 || len_of(p, t) == 0) continue;
+      float M = -INFINITY, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      add_pieces(lane, cta, job.last, p.tile_o, p.tile_ml, 256, i / p.tokens * 128 + i % p.tokens * p.grp + hh, M, L, O);
+      const long long u = p.unit_first[t], units = p.unit_first[t + 1] - u;
+      if (units > 0) {
+        const long long x = u * p.Hkv + job.h * units;
+        const int d0 = (int)divided(x, q), d1 = (int)divided(x + units - 1, q);
+        const size_t place = (size_t)t * p.Hq + hq;
+        if (d0 == d1) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
+        else add_pieces(lane, d0, d1, p.cut_o, p.cut_ml, 8, hh, M, L, O);
+      }
+      const float inv = 1.f / L;
+      store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
     }
-    if (units == 0 ? shared && c0 == c1 : d0 == d1 && !(shared && c0 != c1)) continue;  // written by whom had all of it
+  } else {
+    const int cta = blockIdx.x - p.tile_ctas * kJoinParts;
+    const qeng_own_job job = p.own_jobs[cta];
+    if (job.t < 0 || warp >= p.grp) return;
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (units > 0 && d0 != d1) add_pieces(lane, d0, d1, all, p.own_ctas, p.cut_o, p.cut_ml, 8, hh, M, L, O);
-    if (shared && c0 != c1) {
-      const int i = (t - groups.first[row.group]) % (2 * p.tokens);
-      add_pieces(lane, c0, c1, (long long)p.tile_first[groups.tile[p.G]] * p.Hkv, p.tile_ctas, p.tile_o, p.tile_ml, 256, i / p.tokens * 128 + i % p.tokens * p.grp + hh, M, L, O);
-    }
-    // of the two at most one is whole
-    const size_t place = (size_t)t * p.Hq + hq;
-    if ((shared && c0 == c1) || (units > 0 && d0 == d1)) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
-    const float inv = row.len == 0 ? 0.f : 1.f / L;
-    store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
+    add_pieces(lane, cta, job.last, p.cut_o, p.cut_ml, 8, warp, M, L, O);
+    const int hq = job.h * p.grp + warp;
+    const size_t place = (size_t)job.t * p.Hq + hq;
+    if (job.shared) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
+    const float inv = 1.f / L;
+    store4(p, job.t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
   }
 }
 
@@ -1102,8 +1182,8 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   if (!rows && table_rows < T) return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: a table of %lld rows for %lld without their rows", (long long)table_rows, (long long)T);
   const int grp = (int)(Hq / pool->kv_heads), tokens = 128 / grp;
   const int64_t tiles = (T + 2 * tokens - 1) / (2 * tokens) + (G < T ? G : T);  // at most
-  if (tiles > kSharedTiles || (max_pages / 8 + 2) * tiles > 0x7fffffff)
-    return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: rows / %d + groups exceed %d, or their pages 2^34", 2 * tokens, kSharedTiles);
+  if (tiles > kSharedTiles || (max_pages / 8 + 2) * tiles * pool->kv_heads > 0x7fffffff)
+    return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: rows / %d + groups exceed %d, or those times kv heads and pages 2^34", 2 * tokens, kSharedTiles);
   if (ldq < Hq * kHD || ldo < Hq * kHD) return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: rows of %lld and %lld values hold less than %lld heads", (long long)ldq, (long long)ldo, (long long)Hq);
   if (((reinterpret_cast<uintptr_t>(q_f16) | reinterpret_cast<uintptr_t>(out)) & 15) != 0 || ldq % 8 != 0 || ldo % (out_dtype == QENG_F32 ? 4 : 8) != 0)
     return qeng_fail(ctx, QENG_ERR_ALIGN, "attn_shared: rows of q and out must be 16-byte aligned");
@@ -1131,12 +1211,13 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   rc = tile_maps(ctx, p, &tile_map, &q_map);
   if (rc != QENG_OK) return rc;
   qeng_scratch* sc = qeng_scratch_for(ctx, st);
-  // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml
+  // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml, jobs
   const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_ctas * 8;
-  const size_t need[8] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8};
-  size_t at[9] = {0};
-  for (int i = 0; i < 8; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
-  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[8]);
+  const size_t need[10] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
+                           p.tile_ctas * sizeof(qeng_tile_job), p.own_ctas * sizeof(qeng_own_job)};
+  size_t at[11] = {0};
+  for (int i = 0; i < 10; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
+  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[10]);
   if (rc != QENG_OK) return rc;
   unsigned char* const mem = static_cast<unsigned char*>(sc->shared.ptr);
   p.tile_first = reinterpret_cast<int*>(mem);
@@ -1147,12 +1228,26 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   p.unit_first = reinterpret_cast<long long*>(mem + at[5]);
   p.cut_o = reinterpret_cast<float*>(mem + at[6]);
   p.cut_ml = reinterpret_cast<float*>(mem + at[7]);
+  p.tile_jobs = reinterpret_cast<qeng_tile_job*>(mem + at[8]);
+  p.own_jobs = reinterpret_cast<qeng_own_job*>(mem + at[9]);
   if (out_dtype == QENG_F32) attn_tile_kernel<true><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   else attn_tile_kernel<false><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   QENG_LAUNCH_CHECK(ctx);
-  attn_own_kernel<<<(unsigned)p.own_ctas, kThreads, kOwnSmem + groups_bytes(G), st>>>(p, map);
-  QENG_LAUNCH_CHECK(ctx);
-  attn_join_kernel<<<(unsigned)T, kJoinWarps * 32, groups_bytes(G), st>>>(p);
-  QENG_LAUNCH_CHECK(ctx);
+  // the other two may start as CTAs of the one in front leave
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->pdl ? 1 : 0;
+  cfg.gridDim = dim3((unsigned)p.own_ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kOwnSmem + groups_bytes(G);
+  QENG_CUDA(ctx, cudaLaunchKernelEx(&cfg, attn_own_kernel, p, map));
+  cfg.gridDim = dim3((unsigned)(p.tile_ctas * kJoinParts + p.own_ctas));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
+  QENG_CUDA(ctx, cudaLaunchKernelEx(&cfg, attn_join_kernel, p));
   return QENG_OK;
 }

@@ -8,6 +8,14 @@ constexpr int kSharedGroups = 1024;  // groups of rows in a call
 constexpr int kSharedTiles = 4096;   // and double tiles of them
 constexpr int kOwnWarps = 4;         // of a CTA that reads rows' own pages, and pages of a unit of its work
 
+// What CTAs leave for attn_join_kernel to add up: `last` is the last CTA that has a piece.
+struct qeng_tile_job {
+  int t0, rows, h, last;  // rows of (token, head) of the double tile; none: no job
+};
+struct qeng_own_job {
+  int t, h, last, shared;  // t < 0: no job; shared: the row's shared part is in row_o
+};
+
 struct qeng_shared_attn {
   const __half* q;         // [T] rows of [Hq][128], ldq values apart
   const int32_t* table;    // [table_rows][max_pages]
@@ -23,12 +31,14 @@ struct qeng_shared_attn {
   // Working memory: sums that are not a row's whole result, each with (m, l): the sum is of 2^(x - m) v, l of 2^(x - m).
   //
   // The shared pages of a group are worked on by double tiles: 2 * tokens rows, one kv head, all keys that any of them attends, by blocks
-  // of 128.  The CTAs of attn_tile_kernel divide all blocks evenly (CTA c: [c W / n, (c + 1) W / n) in the order of double tiles, kv
-  // heads, keys), so that a CTA has whole ones but for the first and the last.  The pages that a row has to itself are divided the same way
+  // of 128.  The CTAs of attn_tile_kernel divide all blocks evenly (in the order of double tiles, kv heads,
+  // keys), so that a CTA has whole ones but for the first and the last.  The pages that a row has to itself are divided the same way
   // among the CTAs of attn_own_kernel, in units of four pages.
   int* tile_first;             // [double tiles + 1] blocks (of one kv head) before a double tile
   float *tile_o, *tile_ml;     // cut between CTAs: [2 tile_ctas][256][128], [..][2]: of what a CTA begins with, of what it ends with
   float *row_o, *row_ml;       // [T][Hq][128], [..][2]: the shared part of a row that has pages to itself, whole; or, where that is cut, the row's own, whole
   long long* unit_first;       // [T + 1] units (of one kv head) before a row
+  qeng_tile_job* tile_jobs;    // [tile_ctas]
+  qeng_own_job* own_jobs;      // [own_ctas]
   float *cut_o, *cut_ml;       // cut between CTAs: [2 own_ctas][8][128], [..][2]
 };
