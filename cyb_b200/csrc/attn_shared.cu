@@ -222,10 +222,10 @@ __device__ __forceinline__ void add_pieces(int lane, int c0, int c1, const float
 
 // ---- shared pages -------------------------------------------------------------------------------------------------------------
 // A double tile is two tiles of 128 MMA rows, each of `tokens` tokens x the query heads of a kv head, against the same keys, 128 (eight
-// pages) at a time.  Queries, K and V lie in shared memory, the scores S and the outputs O in tensor memory (256 columns a tile); the
-// weights P take the place of the scores, as one f16 number or two (f32 results).  Warps 0-3 and 4-7 are the softmax of the two tiles, a
-// lane a row; 8 issues the MMAs, 9 the copies, 10 and 11 look for values that are not finite.  The MMAs of one tile run beside the
-// softmax of the other.  O is rescaled only when a row's maximum has grown by more than 2^kGrow since it was last.
+// pages) at a time.  Queries, K and V lie in shared memory, the scores S (two times 64 keys) and the outputs O in tensor memory (256 columns a
+// tile); the weights P take the place of the scores, as one f16 number or two (f32 results).  Warps 0-3 and 4-7 are the softmax of the two tiles, a
+// lane a row; 8 issues the MMAs, 9 the copies, 10 and 11 look for values that are not finite.  The MMAs of 64 keys run beside
+// the softmax of the next and of the other tile.  O is rescaled only when a row's maximum has grown by more than 2^kGrow since it was last.
 //
 // K and V tiles: [2 halves of 64 dims][128 keys][128 bytes], 128-byte swizzled; K is a K-major operand of 128 columns, V an MN-major one.
 constexpr int kRows = 128, kKeys = 128;
@@ -286,8 +286,9 @@ struct TileShared {
   uint32_t bad[2][4];           // of a V tile: keys with a value that is not finite
   int begun[2];                 // O of a tile holds sums before its first MMA
   uint32_t tmem;
-  // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); scores and last outputs of a tile done, weights ready, V looked through
-  uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2], checked[2], drained;
+  // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); of a tile: scores done, values added, the last of a
+  // piece, weights ready (of the first, the second 64 keys); V looked through
+  uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], vdone[2], odone[2], pready[2][2], checked[2], drained;
 };
 
 // cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
@@ -309,8 +310,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       mbar_init(smem_u32(sh.pfull + i), 1);
       mbar_init(smem_u32(sh.pempty + i), kSoftWarps + 1 + kCheckWarps);
       mbar_init(smem_u32(sh.sdone + i), 1);
+      for (int k = 0; k < 2; ++k) mbar_init(smem_u32(&sh.pready[i][k]), kSoftWarps / 2);
+      mbar_init(smem_u32(sh.vdone + i), 1);
       mbar_init(smem_u32(sh.odone + i), 1);
-      mbar_init(smem_u32(sh.pready + i), kSoftWarps / 2);
       mbar_init(smem_u32(sh.checked + i), kCheckWarps);
     }
     for (int i = 0; i < 4; ++i) {
@@ -467,64 +469,80 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     // f16 x f16 -> f32, M = N = 128; B of S K-major, of O MN-major
     constexpr uint32_t kIdescS = (1u << 4) | (16u << 17) | (8u << 24), kIdescO = kIdescS | (1u << 16);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, qs, 0), r0 = __shfl_sync(0xffffffffu, ring, 0);
-    int b = 0;                         // blocks so far
-    uint32_t turn[2] = {0, 0}, edges[2] = {0, 0};  // blocks of a tile; edges among the even and odd V tiles
+    int b = 0;                // blocks so far
+    uint32_t turn = 0;        // parities of pready (bit 2 x + half) and of checked (bit 4 + slot)
     const bool leader = elect_one();
     const int who = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
     Piece w;
     while (next_piece(w)) {
       bool lost = false;
       if (leader) {
-        const auto scores = [&](int x, int blk) {
-          const uint64_t a = make_desc(q0 + (uint32_t)x * kTileBytes, 16, 1024), k = make_desc(r0 + (uint32_t)(2 * (blk & 1)) * kTileBytes, 16, 1024);
+        const auto full = [&](int kv, int blk) { return mbar_wait(smem_u32(sh.full + 2 * (blk & 1) + kv), (uint32_t)(blk >> 1) & 1u); };
+        const auto scores = [&](int x, int blk, bool last) {
+          const uint32_t slot = 2u * (blk & 1);
+          const uint64_t a = make_desc(q0 + (uint32_t)x * kTileBytes, 16, 1024), k = make_desc(r0 + slot * kTileBytes, 16, 1024);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t at = (uint32_t)(i >> 2) * (kHalf >> 4) + (uint32_t)(i & 3) * 2u;
-            umma_ss(tm + (uint32_t)x * 256u, a + at, k + at, kIdescS, i > 0);
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t at = (uint32_t)(c >> 2) * (kHalf >> 4) + (uint32_t)(c & 3) * 2u;
+            umma_ss(tm + (uint32_t)x * 256u, a + at, k + at, kIdescS, c > 0);
           }
           umma_commit(smem_u32(sh.sdone + x));
+          if (x + 1 == w.tiles) {
+            umma_commit(smem_u32(sh.empty + slot));
+            if (last) umma_commit(smem_u32(&sh.qempty));
+          }
         };
-        const auto full = [&](int kv, int blk) { return mbar_wait(smem_u32(sh.full + 2 * (blk & 1) + kv), (uint32_t)(blk >> 1) & 1u); };
         lost = !mbar_wait(smem_u32(&sh.qfull), (uint32_t)(npiece - 1) & 1u) || !full(0, b);
         if (!lost) {
           fence_after();
-          for (int x = 0; x < w.tiles; ++x) scores(x, b);
-          umma_commit(smem_u32(sh.empty + 2 * (b & 1)));
-          if (w.blocks == 1) umma_commit(smem_u32(&sh.qempty));
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (x < w.tiles) scores(x, b, w.blocks == 1);
         }
         for (int j = 0; j < w.blocks && !lost; ++j) {
-          const int blk = b + j, steps = min(8, (w.kv1 - (w.page0 + 8 * j) * kPage + kPage - 1) / kPage);
-          const bool edge = is_edge(w, j), more = j + 1 < w.blocks;
-          for (int x = 0; x < w.tiles; ++x) {
-            if (!mbar_wait(smem_u32(sh.pready + x), turn[x] & 1u)) { lost = true; break; }
-            ++turn[x];
-            if (x == 0) {
-              if (!full(1, blk)) { lost = true; break; }
-              if (edge && !mbar_wait(smem_u32(sh.checked + (blk & 1)), edges[blk & 1] & 1u)) { lost = true; break; }
-              edges[blk & 1] += edge;
-            }
-            fence_after();
+          const int blk = b + j, left = w.kv1 - (w.page0 + 8 * j) * kPage;
+          const bool more = j + 1 < w.blocks;
+          const uint32_t slot = 2u * (blk & 1) + 1u;
+          const uint64_t v = make_desc(r0 + slot * kTileBytes, kHalf, 1024);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (x >= w.tiles) continue;
             const uint32_t o = tm + (uint32_t)x * 256u + kO, a = tm + (uint32_t)x * 256u;
-            const uint64_t v = make_desc(r0 + (uint32_t)(2 * (blk & 1) + 1) * kTileBytes, kHalf, 1024);
-            uint32_t acc = j > 0 || *(volatile int*)&sh.begun[x];
-            for (int k = 0; k < steps; ++k) {
-              const uint32_t w_at = a + 64u * (k >> 2) + 8u * (k & 3);
-              umma_ts(o, w_at, v + (uint32_t)k * (2048u >> 4), kIdescO, acc);
-              if (kTwo) umma_ts(o, w_at + 32u, v + (uint32_t)k * (2048u >> 4), kIdescO, 1u);
-              acc = 1u;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (lost || left <= 64 * half) continue;
+              if (!mbar_wait(smem_u32(&sh.pready[x][half]), (turn >> (2 * x + half)) & 1u)) { lost = true; continue; }
+              turn ^= 1u << (2 * x + half);
+              if (x == 0 && half == 0) {
+                if (!full(1, blk)) { lost = true; continue; }
+                if (is_edge(w, j)) {
+                  if (!mbar_wait(smem_u32(sh.checked + (blk & 1)), (turn >> (4 + (blk & 1))) & 1u)) { lost = true; continue; }
+                  turn ^= 16u << (blk & 1);
+                }
+              }
+              fence_after();
+              uint32_t acc = half > 0 || j > 0 || *(volatile int*)&sh.begun[x];
+              const int steps = (left - 64 * half + kPage - 1) / kPage;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (k >= steps) continue;
+                umma_ts(o, a + 64u * half + 8u * k, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, acc);
+                if (kTwo) umma_ts(o, a + 64u * half + 32u + 8u * k, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, 1u);
+                acc = 1u;
+              }
+              umma_commit(smem_u32(sh.vdone + x));
             }
-            if (x + 1 == w.tiles) umma_commit(smem_u32(sh.empty + 2 * (blk & 1) + 1));
+            if (lost) continue;
+            if (x + 1 == w.tiles) umma_commit(smem_u32(sh.empty + slot));
             if (!more) {
               umma_commit(smem_u32(sh.odone + x));
               continue;
             }
-            if (x == 0 && !full(0, blk + 1)) { lost = true; break; }
-            fence_after();
-            scores(x, blk + 1);
-            if (x + 1 == w.tiles) {
-              umma_commit(smem_u32(sh.empty + 2 * ((blk + 1) & 1)));
-              if (j + 2 == w.blocks) umma_commit(smem_u32(&sh.qempty));
+            if (x == 0) {
+              if (!full(0, blk + 1)) { lost = true; continue; }
+              fence_after();
             }
+            scores(x, blk + 1, j + 2 == w.blocks);
           }
         }
         if (lost) {  // what was issued still has to finish before tensor memory is freed
@@ -593,11 +611,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     const float sc = p.softcap > 0.f ? 1.f : p.scale * kLog2e;
     const float cap2 = 2.f * kLog2e * p.scale / p.softcap, cap = p.softcap * kLog2e;
     int b = 0;
-    uint32_t turn = 0, ends = 0, edges[2] = {0, 0};
+    uint32_t n = 0, turn = 0;  // 64 keys at a time so far; parities of sdone (bit 0), odone (1) and checked (4 + slot)
     Piece w;
     while (next_piece(w) && !failed) {
       if (x >= w.tiles) {
-        for (int j = 0; j < w.blocks; ++j) edges[(b + j) & 1] += is_edge(w, j);
+        for (int j = 0; j < w.blocks; ++j)
+          if (is_edge(w, j)) turn ^= 16u << ((b + j) & 1);
         b += w.blocks;
         continue;
       }
@@ -613,38 +632,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       // a row that attends none of these keys attends everything, to nobody's use
       const int begin = some ? win0 : 0, end = some ? min(len, w.keys) : 0x7fffffff;
       float m_run = -INFINITY, l_run = 0.f;
+      const int halves = (min(w.kv1 - w.page0 * kPage, w.blocks * kKeys) + 63) / 64;
 #pragma unroll 1
-      for (int j = 0; j < w.blocks; ++j, ++b) {
-        const int key0 = (w.page0 + 8 * j) * kPage;
-        const bool edge = is_edge(w, j);
-        if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
-        fence_after();
-        // 64 keys at a time: the first half's scores are read twice, once for the maximum
+      for (int k64 = 0; k64 < halves; ++k64, ++n) {  // 64 keys at a time
+        const int key0 = w.page0 * kPage + 64 * k64, blk = b + (k64 >> 1);
+        const bool edge = is_edge(w, k64 >> 1);
+        const uint32_t at = mem + 64u * (k64 & 1);
+        if ((k64 & 1) == 0) {
+          if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
+          turn ^= 1u;
+          fence_after();
+        }
         float s[64];
-        const auto masked = [&](int half) {
-          if (!edge) return;
-          const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
+        tmem_ld64(at, reinterpret_cast<uint32_t*>(s));
+        if (p.softcap > 0.f) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
+        }
+        if (edge) {
+          const int e = end - key0, a = begin - key0;
 #pragma unroll
           for (int k = 0; k < 64; ++k)
             if (k >= e || k < a) s[k] = -INFINITY;
-        };
-        float mx = -INFINITY;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
-          masked(half);
-          float mx4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int k = 0; k < 64; ++k) mx4[k & 3] = fmaxf(mx4[k & 3], s[k]);
-          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         }
-        if (p.softcap > 0.f && mx != -INFINITY) mx = capped(mx, cap2, cap);
+        float mx4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int k = 4; k < 64; k += 2) mx4[(k >> 1) & 3] = max3(mx4[(k >> 1) & 3], s[k], s[k + 1]);
+        const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
         // the reference of the row's weights moves when its maximum has left it far behind
         const bool moved = mx > m_run && (m_run == -INFINITY || (mx - m_run) * sc > kGrow);
         const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
         if (moved) m_run = mx;
         l_run *= alpha;
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // O is added to by what the last weights were multiplied with; nothing behind it is issued before this warp's next arrival
+        const auto settled = [&] {
+          if (k64 > 0 && !wait_warp(smem_u32(sh.vdone + x), (n - 1) & 1u)) failed = true;
+          fence_after();
+        };
+        if (k64 > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          settled();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
@@ -659,48 +685,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.f;
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-          if (half == 0) {
-            tmem_ld64(mem, reinterpret_cast<uint32_t*>(s));
-            if (!(p.softcap > 0.f)) masked(0);
-          }
-          if (p.softcap > 0.f) {
+        for (int c = 0; c < 2; ++c) {  // 32 keys at a time
+          uint32_t hi[16], lo[16];
 #pragma unroll
-            for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
-            masked(half);
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {  // 32 keys at a time
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
-              fma2(a0, a1, sc, off);
-              a0 = ex2(a0);
-              a1 = ex2(a1);
-              add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
-              hi[k] = pack_h2(a0, a1);
-              if (kTwo) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-                lo[k] = pack_h2(a0 - f.x, a1 - f.y);
-              }
+          for (int k = 0; k < 16; ++k) {
+            float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
+            fma2(a0, a1, sc, off);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
+            hi[k] = pack_h2(a0, a1);
+            if (kTwo) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+              lo[k] = pack_h2(a0 - f.x, a1 - f.y);
             }
-            tmem_st16(mem + 64 * half + 16 * c, hi);
-            if (kTwo) tmem_st16(mem + 64 * half + 32 + 16 * c, lo);
           }
+          tmem_st16(at + 16 * c, hi);
+          if (kTwo) tmem_st16(at + 32 + 16 * c, lo);
         }
         l_run += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         st_wait();
         bool zeroed = false;
         if (edge) {
-          if (!wait_warp(smem_u32(sh.checked + (b & 1)), edges[b & 1] & 1u)) { failed = true; break; }
-          ++edges[b & 1];
+          if ((k64 & 1) == 0) {
+            if (!wait_warp(smem_u32(sh.checked + (blk & 1)), (turn >> (4 + (blk & 1))) & 1u)) { failed = true; break; }
+            turn ^= 16u << (blk & 1);
+          }
+          bool first = true;
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
 #pragma unroll 1
-            for (uint32_t mask = sh.bad[b & 1][q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
+            for (uint32_t mask = sh.bad[blk & 1][2 * (k64 & 1) + q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
               const int k = 32 * q + __ffs(mask) - 1, key = key0 + k;
-              if (j == 0 && !zeroed) {
+              if (first && k64 > 0) settled();
+              if (first && k64 == 0) {
                 uint32_t z[32];
 #pragma unroll
                 for (int d = 0; d < 32; ++d) z[d] = 0u;
@@ -709,10 +727,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
                 st_wait();
                 zeroed = true;
               }
+              first = false;
               float weight = 0.f;
 #pragma unroll 1
               for (int c = 0; c <= (kTwo ? 32 : 0); c += 32) {
-                const uint32_t y = tmem_ld1(mem + (k & 64) + c + (k & 63) / 2);
+                const uint32_t y = tmem_ld1(at + c + k / 2);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
                 weight += k & 1 ? f.y : f.x;
               }
@@ -742,21 +761,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (j == 0 && (warp & 3) == 0) *(volatile int*)&sh.begun[x] = zeroed;
-          mbar_arrive(smem_u32(sh.pready + x));
+          if (k64 == 0 && (warp & 3) == 0) *(volatile int*)&sh.begun[x] = zeroed;
+          mbar_arrive(smem_u32(&sh.pready[x][k64 & 1]));
         }
-        ++turn;
       }
-      if (failed || !wait_warp(smem_u32(sh.odone + x), ends & 1u)) { failed = true; break; }
-      ++ends;
+      b += w.blocks;
+      if (failed || !wait_warp(smem_u32(sh.odone + x), (turn >> 1) & 1u)) { failed = true; break; }
+      turn ^= 2u;
       fence_after();
       // Whole and all that the row attends: its result.  Otherwise what has to be added to others' sums.
       const bool alone = max((len + kPage - 1) / kPage - max(win0 / kPage, w.keys / kPage), 0) == 0;
       const bool result = w.whole && alone;  // (attn_own_kernel writes the zeros of a row that attends nothing)
       const float inv = 1.f / l_run;
-      const size_t at = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
+      const size_t place = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
       if (live && !(w.whole && alone)) {
-        float* const ml = (w.whole ? p.row_ml : p.tile_ml) + 2 * at;
+        float* const ml = (w.whole ? p.row_ml : p.tile_ml) + 2 * place;
         // rows that attend nothing here have no weight
         *reinterpret_cast<float2*>(ml) = some ? make_float2(m_run == -INFINITY ? -INFINITY : m_run * sc - kHigh, l_run) : make_float2(-INFINITY, 0.f);
       }
@@ -775,7 +794,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
             store8(p, t, head, 32 * c + d, f);
           }
         } else {
-          float4* const dst = reinterpret_cast<float4*>((w.whole ? p.row_o : p.tile_o) + at * kHD + 32 * c);
+          float4* const dst = reinterpret_cast<float4*>((w.whole ? p.row_o : p.tile_o) + place * kHD + 32 * c);
 #pragma unroll
           for (int d = 0; d < 8; ++d) dst[d] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
         }
