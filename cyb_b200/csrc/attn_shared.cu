@@ -20,7 +20,6 @@ constexpr int kThreads = kOwnWarps * 32, kDepth = 2, kRing = kDepth * kOwnWarps;
 constexpr uint32_t kSlotBytes = 2 * kPage * kHD * 2;
 constexpr int kHDP = kHD + 4;  // row stride of the warps' sums in shared memory: no bank conflicts
 constexpr size_t kOwnSmem = kRing * kSlotBytes + 1024;
-constexpr int kChunks = 512;     // of rows, whose units are counted together
 constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row is 2^kHigh and more: the smallest that a f16 number holds at full precision is then 2^-21 of it.
 constexpr float kHigh = 7.f;
@@ -156,13 +155,13 @@ __device__ __forceinline__ Row row_of(const qeng_shared_attn& p, const Groups& g
   r.pages = max(0, (r.len + kPage - 1) / kPage - r.page0);
   return r;
 }
-__device__ __forceinline__ int units_of(const Row& r) { return (r.pages + kOwnWarps - 1) / kOwnWarps; }
-
-// The CTAs of a kernel divide its work evenly: CTA c has the units [c q, (c + 1) q) of `all`, q = share(all, n).
+// The CTAs (or warps) of a kernel divide its work evenly: CTA c has the units [c q, (c + 1) q) of `all`, q = share(all, n).
 __device__ __forceinline__ long long divided(long long x, long long q) {  // of numbers that are not negative; most fit 32 bits
   return ((unsigned long long)(x | q) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)q) : x / q;
 }
-__device__ __forceinline__ long long share(long long all, int n) { return max(divided(all + n - 1, n), 1ll); }
+__device__ __forceinline__ long long share(long long all, int n, int least = 1) { return max(divided(all + n - 1, n), (long long)least); }
+constexpr int kLeast = 4;  // pages of a warp of attn_own_kernel at least: cutting a pair costs more than reading that many
+__device__ __forceinline__ long long own_share(const qeng_shared_attn& p) { return share(p.unit_first[p.T] * p.Hkv, p.own_warps, kLeast); }
 
 // Adds up to 32 sums of one (row, head) to a running (M, L, O): lane i has the i-th, if any; its (m, l) and the place of its 128 values.
 // The lanes' pairs are loaded together and so are the values, four dims a lane.
@@ -233,7 +232,7 @@ constexpr uint32_t kTileBytes = kRows * kHD * 2, kHalf = kTileBytes / 2;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + 1, kCheckWarp = kLoadWarp + 1, kCheckWarps = 2;
 constexpr int kTileThreads = (kCheckWarp + kCheckWarps) * 32;
 constexpr size_t kTileSmem = 6 * kTileBytes + 1024;
-// Columns of a tile: scores at 0; the weights of 64 keys take the place of their scores, the second terms 32 columns behind the first.
+// Columns of a tile: scores at 0; the weights of 32 keys take the place of their scores, the second terms 16 columns behind the first.
 constexpr uint32_t kO = 128;
 constexpr float kGrow = 8.f;   // weights reach 2^(kHigh + kGrow), below the largest f16 number
 
@@ -280,15 +279,46 @@ __device__ __forceinline__ void rows_of_tile(const qeng_shared_attn& p, const Gr
 }
 __device__ __forceinline__ int blocks_of(int kv0, int kv1) { return kv1 > kv0 ? (kv1 - kv0 / kPage * kPage + kKeys - 1) / kKeys : 0; }
 
+// unit_first, by one CTA
+__device__ __forceinline__ void count_units(const qeng_shared_attn& p, const Groups& g, long long* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long before = 0;
+  for (int t0 = 0; t0 < p.T; t0 += kTileThreads) {
+    const int t = t0 + threadIdx.x;
+    long long n = 0;
+    if (t < p.T) {
+      n = row_of(p, g, t).pages;
+      if (p.rows && t >= g.first[0] && t < g.first[p.G] && __ldg(p.rows + t) >= p.table_rows) atomicExch(p.status, 6);
+    }
+    long long x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    long long front = before;
+    for (int w = 0; w < kTileThreads / 32; ++w) {
+      const long long y = sums[w];
+      if (w < warp) front += y;
+      before += y;
+    }
+    if (t < p.T) p.unit_first[t] = front + x - n;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.unit_first[p.T] = before;
+}
+
 struct TileShared {
-  int first[kSharedTiles + 1];  // blocks (of one kv head) before a double tile
+  alignas(8) int first[kSharedTiles + 1];  // blocks (of one kv head) before a double tile
   Piece piece[2];
   uint32_t bad[2][4];           // of a V tile: keys with a value that is not finite
   int begun[2];                 // O of a tile holds sums before its first MMA
   uint32_t tmem;
-  // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); of a tile: scores done, values added, the last of a
-  // piece, weights ready (of the first, the second 64 keys); V looked through
-  uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], vdone[2], odone[2], pready[2][2], checked[2], drained;
+  // full / empty: pieces' descriptions, queries, K and V tiles (even, odd); of a tile: scores done, the last values of a piece
+  // added, weights ready (of the first, the second 64 keys); V looked through
+  uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2][2], checked[2], drained;
 };
 
 // cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
@@ -311,7 +341,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       mbar_init(smem_u32(sh.pempty + i), kSoftWarps + 1 + kCheckWarps);
       mbar_init(smem_u32(sh.sdone + i), 1);
       for (int k = 0; k < 2; ++k) mbar_init(smem_u32(&sh.pready[i][k]), kSoftWarps / 2);
-      mbar_init(smem_u32(sh.vdone + i), 1);
       mbar_init(smem_u32(sh.odone + i), 1);
       mbar_init(smem_u32(sh.checked + i), kCheckWarps);
     }
@@ -324,8 +353,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     mbar_init(smem_u32(&sh.drained), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (tid == 0) p.tile_jobs[cta].rows = 0;
+  if (tid == 0) p.tile_jobs[cta].tokens = 0;
+  if (warp == kLoadWarp && lane < 2) asm volatile("prefetch.tensormap [%0];\n" ::"l"(lane == 0 ? &kvmap : &qmap) : "memory");
   if (!read_groups(p, groups)) return;  // (attn_own_kernel reports it)
+  if (cta == (int)gridDim.x - 1) count_units(p, groups, reinterpret_cast<long long*>(sh.first));  // it has least to do
   const int ntiles = groups.tile[p.G];
   {  // keys that the double tiles attend, a thread a row; the ring is not in use yet
     int* const kv0 = reinterpret_cast<int*>(smem_raw);
@@ -375,19 +406,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
   const int all = sh.first[ntiles] * p.Hkv, q = (int)share(all, gridDim.x), u0 = min(all, cta * q), u1 = min(all, u0 + q);
   bool failed = false;
 
-  // what a warp of another role does for the next piece's description; false: no more
+  // a warp of another role asks for the next piece's description, which stays until it asks again; null: no more
   int npiece = 0;
-  const auto next_piece = [&](Piece& w) {
-    const int e = npiece & 1;
-    if (!wait_warp(smem_u32(sh.pfull + e), (uint32_t)(npiece >> 1) & 1u)) {
-      failed = true;
-      return false;
+  const auto next_piece = [&]() -> const Piece* {
+    if (npiece > 0) {  // done with the last one
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(sh.pempty + ((npiece - 1) & 1)));
     }
-    w = sh.piece[e];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(sh.pempty + e));
+    const int e = npiece & 1;
+    if (failed || !wait_warp(smem_u32(sh.pfull + e), (uint32_t)(npiece >> 1) & 1u)) {
+      failed = true;
+      return nullptr;
+    }
     ++npiece;
-    return w.blocks > 0;
+    return sh.piece[e].blocks > 0 ? &sh.piece[e] : nullptr;
   };
 
   if (warp == kLoadWarp) {
@@ -413,7 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           job.t0 = w.t0;
           job.h = w.h;
           job.last = (u + nb - 1) / q;
-          job.rows = w.ntok * p.grp;
+          job.tokens = w.ntok;
         }
       }
       if (!wait_warp(smem_u32(sh.pempty + (n & 1)), ((uint32_t)(n >> 1) & 1u) ^ 1u)) { failed = true; break; }
@@ -427,6 +459,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       const int32_t* const ids = p.table + (size_t)w.table_row * p.max_pages;
       // lanes 2 i and 2 i + 1 copy the two halves of page i of the block
       const int pg = lane >> 1, half = lane & 1;
+      const auto queries = [&] {  // half a tile at a time
+        if (!wait_warp(smem_u32(&sh.qempty), ((uint32_t)n & 1u) ^ 1u)) {
+          failed = true;
+          return;
+        }
+        if (lane == 0) mbar_expect_tx(smem_u32(&sh.qfull), (uint32_t)(w.tiles * 2 * 128 * p.grp * p.tokens));
+        __syncwarp();
+        if (lane < 2 * w.tiles)
+          asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                           qs + (uint32_t)(lane >> 1) * kTileBytes + (uint32_t)half * kHalf),
+                       "l"(&qmap), "r"(64 * half), "r"(w.h * p.grp), "r"(w.t0 + (lane >> 1) * p.tokens), "r"(smem_u32(&sh.qfull))
+                       : "memory");
+      };
+      if (n == 0) queries();
       int id = lane < 16 && w.page0 + pg <= last_page ? ids[w.page0 + pg] : 0;
       for (int j = 0; j < w.blocks && !failed; ++j, ++b) {
         const int here = w.page0 + j * 8, pages = min(8, last_page - here + 1);
@@ -449,16 +495,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
                          "l"(&kvmap), "r"(0), "r"(row + 16 * kv), "r"(half), "r"(bar)
                          : "memory");
         }
-        if (j == 0 && !failed) {  // queries: half a tile at a time
-          if (!wait_warp(smem_u32(&sh.qempty), ((uint32_t)n & 1u) ^ 1u)) { failed = true; break; }
-          if (lane == 0) mbar_expect_tx(smem_u32(&sh.qfull), (uint32_t)(w.tiles * 2 * 128 * p.grp * p.tokens));
-          __syncwarp();
-          if (lane < 2 * w.tiles)
-            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
-                             qs + (uint32_t)(lane >> 1) * kTileBytes + (uint32_t)half * kHalf),
-                         "l"(&qmap), "r"(64 * half), "r"(w.h * p.grp), "r"(w.t0 + (lane >> 1) * p.tokens), "r"(smem_u32(&sh.qfull))
-                         : "memory");
-        }
+        if (j == 0 && n > 0 && !failed) queries();  // behind the first K and V: the last piece may still use theirs
       }
       if (failed) break;
       u += w.blocks;
@@ -468,81 +505,81 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     // ===== MMA issue ====================================================================================================
     // f16 x f16 -> f32, M = N = 128; B of S K-major, of O MN-major
     constexpr uint32_t kIdescS = (1u << 4) | (16u << 17) | (8u << 24), kIdescO = kIdescS | (1u << 16);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q0 = __shfl_sync(0xffffffffu, qs, 0), r0 = __shfl_sync(0xffffffffu, ring, 0);
+    constexpr uint32_t kTwoTiles = 2 * kTileBytes >> 4;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), r0 = __shfl_sync(0xffffffffu, ring, 0);
+    const uint64_t qd = make_desc(__shfl_sync(0xffffffffu, qs, 0), 16, 1024);
+    const uint64_t kd = make_desc(r0, 16, 1024), vd = make_desc(r0 + kTileBytes, kHalf, 1024);  // + 2 tiles in the odd blocks
     int b = 0;                // blocks so far
     uint32_t turn = 0;        // parities of pready (bit 2 x + half) and of checked (bit 4 + slot)
     const bool leader = elect_one();
     const int who = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
-    Piece w;
-    while (next_piece(w)) {
+    while (const Piece* const piece = next_piece()) {
+      const int blocks = piece->blocks, tiles = piece->tiles, left0 = piece->kv1 - piece->page0 * kPage;
       bool lost = false;
       if (leader) {
         const auto full = [&](int kv, int blk) { return mbar_wait(smem_u32(sh.full + 2 * (blk & 1) + kv), (uint32_t)(blk >> 1) & 1u); };
         const auto scores = [&](int x, int blk, bool last) {
-          const uint32_t slot = 2u * (blk & 1);
-          const uint64_t a = make_desc(q0 + (uint32_t)x * kTileBytes, 16, 1024), k = make_desc(r0 + slot * kTileBytes, 16, 1024);
+          const uint64_t q = qd + (kTileBytes >> 4) * x, k = kd + kTwoTiles * (blk & 1);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const uint32_t at = (uint32_t)(c >> 2) * (kHalf >> 4) + (uint32_t)(c & 3) * 2u;
-            umma_ss(tm + (uint32_t)x * 256u, a + at, k + at, kIdescS, c > 0);
+            umma_ss(tm + (uint32_t)x * 256u, q + at, k + at, kIdescS, c > 0);
           }
           umma_commit(smem_u32(sh.sdone + x));
-          if (x + 1 == w.tiles) {
-            umma_commit(smem_u32(sh.empty + slot));
+          if (x + 1 == tiles) {
+            umma_commit(smem_u32(sh.empty + 2 * (blk & 1)));
             if (last) umma_commit(smem_u32(&sh.qempty));
           }
         };
         lost = !mbar_wait(smem_u32(&sh.qfull), (uint32_t)(npiece - 1) & 1u) || !full(0, b);
         if (!lost) {
           fence_after();
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (x < w.tiles) scores(x, b, w.blocks == 1);
+          scores(0, b, blocks == 1);
+          if (tiles == 2) scores(1, b, blocks == 1);
         }
-        for (int j = 0; j < w.blocks && !lost; ++j) {
-          const int blk = b + j, left = w.kv1 - (w.page0 + 8 * j) * kPage;
-          const bool more = j + 1 < w.blocks;
-          const uint32_t slot = 2u * (blk & 1) + 1u;
-          const uint64_t v = make_desc(r0 + slot * kTileBytes, kHalf, 1024);
+        for (int j = 0; j < blocks && !lost; ++j) {
+          const int blk = b + j, left = left0 - kKeys * j;
+          const bool edge = is_edge(*piece, j);
+          const uint64_t v = vd + kTwoTiles * (blk & 1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (x >= w.tiles) continue;
-            const uint32_t o = tm + (uint32_t)x * 256u + kO, a = tm + (uint32_t)x * 256u;
+            if (x >= tiles || lost) continue;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 1; half >= 0; --half) {  // the second 64 keys first
               if (lost || left <= 64 * half) continue;
+              const bool first = half == 1 || left <= 64;
               if (!mbar_wait(smem_u32(&sh.pready[x][half]), (turn >> (2 * x + half)) & 1u)) { lost = true; continue; }
               turn ^= 1u << (2 * x + half);
-              if (x == 0 && half == 0) {
+              if (x == 0 && first) {
                 if (!full(1, blk)) { lost = true; continue; }
-                if (is_edge(w, j)) {
+                if (edge) {
                   if (!mbar_wait(smem_u32(sh.checked + (blk & 1)), (turn >> (4 + (blk & 1))) & 1u)) { lost = true; continue; }
                   turn ^= 16u << (blk & 1);
                 }
               }
               fence_after();
-              uint32_t acc = half > 0 || j > 0 || *(volatile int*)&sh.begun[x];
+              uint32_t acc = !first || j > 0 || *(volatile int*)&sh.begun[x];
               const int steps = (left - 64 * half + kPage - 1) / kPage;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 if (k >= steps) continue;
-                umma_ts(o, a + 64u * half + 8u * k, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, acc);
-                if (kTwo) umma_ts(o, a + 64u * half + 32u + 8u * k, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, 1u);
+                const uint32_t w_at = tm + (uint32_t)x * 256u + 64u * half + 32u * (k >> 1) + 8u * (k & 1);
+                umma_ts(tm + (uint32_t)x * 256u + kO, w_at, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, acc);
+                if (kTwo) umma_ts(tm + (uint32_t)x * 256u + kO, w_at + 16u, v + (uint32_t)(4 * half + k) * (2048u >> 4), kIdescO, 1u);
                 acc = 1u;
               }
-              umma_commit(smem_u32(sh.vdone + x));
             }
             if (lost) continue;
-            if (x + 1 == w.tiles) umma_commit(smem_u32(sh.empty + slot));
-            if (!more) {
+            if (j + 1 < blocks) {
+              if (x == 0) {
+                if (!full(0, blk + 1)) { lost = true; continue; }
+                fence_after();
+              }
+              scores(x, blk + 1, j + 2 == blocks);
+            } else {
               umma_commit(smem_u32(sh.odone + x));
-              continue;
             }
-            if (x == 0) {
-              if (!full(0, blk + 1)) { lost = true; continue; }
-              fence_after();
-            }
-            scores(x, blk + 1, j + 2 == w.blocks);
+            if (x + 1 == tiles) umma_commit(smem_u32(sh.empty + 2 * (blk & 1) + 1));
           }
         }
         if (lost) {  // what was issued still has to finish before tensor memory is freed
@@ -552,7 +589,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       }
       lost = __shfl_sync(0xffffffffu, (int)lost, who);
       if (lost) { failed = true; break; }
-      b += w.blocks;
+      b += blocks;
     }
   } else if (warp >= kCheckWarp) {
     // ===== values that are not finite ===================================================================================
@@ -560,8 +597,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     // is zero, but zero times infinity is NaN).  Such keys are cleared here, and their rows added by the softmax; keys that nobody
     // attends, and what no copy wrote, are cleared, too.
     int b = 0;
-    Piece w;
-    while (next_piece(w) && !failed) {
+    while (const Piece* const piece = next_piece()) {
+      const Piece& w = *piece;
       for (int j = 0; j < w.blocks && !failed; ++j, ++b) {
         // every tile is waited for, and let go: a parity says nothing to those who have missed a turn
         if (!wait_warp(smem_u32(sh.full + 2 * (b & 1) + 1), (uint32_t)(b >> 1) & 1u)) { failed = true; break; }
@@ -611,9 +648,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     const float sc = p.softcap > 0.f ? 1.f : p.scale * kLog2e;
     const float cap2 = 2.f * kLog2e * p.scale / p.softcap, cap = p.softcap * kLog2e;
     int b = 0;
-    uint32_t n = 0, turn = 0;  // 64 keys at a time so far; parities of sdone (bit 0), odone (1) and checked (4 + slot)
-    Piece w;
-    while (next_piece(w) && !failed) {
+    uint32_t turn = 0;  // parities of sdone (bit 0), odone (1) and checked (4 + slot)
+    while (const Piece* const piece = next_piece()) {
+      const Piece& w = *piece;
       if (x >= w.tiles) {
         for (int j = 0; j < w.blocks; ++j)
           if (is_edge(w, j)) turn ^= 16u << ((b + j) & 1);
@@ -632,93 +669,106 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       // a row that attends none of these keys attends everything, to nobody's use
       const int begin = some ? win0 : 0, end = some ? min(len, w.keys) : 0x7fffffff;
       float m_run = -INFINITY, l_run = 0.f;
-      const int halves = (min(w.kv1 - w.page0 * kPage, w.blocks * kKeys) + 63) / 64;
 #pragma unroll 1
-      for (int k64 = 0; k64 < halves; ++k64, ++n) {  // 64 keys at a time
-        const int key0 = w.page0 * kPage + 64 * k64, blk = b + (k64 >> 1);
-        const bool edge = is_edge(w, k64 >> 1);
-        const uint32_t at = mem + 64u * (k64 & 1);
-        if ((k64 & 1) == 0) {
-          if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
-          turn ^= 1u;
-          fence_after();
-        }
+      for (int j = 0; j < w.blocks; ++j, ++b) {
+        const int key0 = (w.page0 + 8 * j) * kPage;
+        const bool edge = is_edge(w, j);
+        if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
+        turn ^= 1u;
+        fence_after();
+        const bool two = key0 + 64 < w.kv1;  // keys in the second half, too
+        // 64 keys at a time, the second ones first.  The first ones' scores are read twice: what was handed over then runs beside
+        // their weights, where the compiler would otherwise put those in front.
         float s[64];
-        tmem_ld64(at, reinterpret_cast<uint32_t*>(s));
-        if (p.softcap > 0.f) {
+        const auto scores = [&](int half) {
+          tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
+          if (p.softcap > 0.f) {
 #pragma unroll
-          for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
+            for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
+          }
+          if (edge) {
+            const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
+#pragma unroll
+            for (int k = 0; k < 64; ++k)
+              if (k >= e || k < a) s[k] = -INFINITY;
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half <= (two ? 1 : 0); ++half) {
+          scores(half);
+          float mx4[4] = {max3(mx, s[0], s[1]), s[2], s[3], max3(s[4], s[5], s[6])};
+#pragma unroll
+          for (int k = 7; k < 63; k += 2) mx4[(k >> 1) & 3] = max3(mx4[(k >> 1) & 3], s[k], s[k + 1]);
+          mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], s[63]);
         }
-        if (edge) {
-          const int e = end - key0, a = begin - key0;
-#pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (k >= e || k < a) s[k] = -INFINITY;
-        }
-        float mx4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int k = 4; k < 64; k += 2) mx4[(k >> 1) & 3] = max3(mx4[(k >> 1) & 3], s[k], s[k + 1]);
-        const float mx = fmaxf(max3(mx4[0], mx4[1], mx4[2]), mx4[3]);
         // the reference of the row's weights moves when its maximum has left it far behind
         const bool moved = mx > m_run && (m_run == -INFINITY || (mx - m_run) * sc > kGrow);
-        const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
-        if (moved) m_run = mx;
-        l_run *= alpha;
-        // O is added to by what the last weights were multiplied with; nothing behind it is issued before this warp's next arrival
-        const auto settled = [&] {
-          if (k64 > 0 && !wait_warp(smem_u32(sh.vdone + x), (n - 1) & 1u)) failed = true;
-          fence_after();
-        };
-        if (k64 > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          settled();
+        if (__any_sync(0xffffffffu, moved)) {
+          const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
+          if (moved) m_run = mx;
+          l_run *= alpha;
+          if (j > 0) {  // the values of the block before are in (its scores came behind them), the next wait for this warp
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(mem + kO + 32 * c, o);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(mem + kO + 32 * c, o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(mem + kO + 32 * c, o);
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st32(mem + kO + 32 * c, o);
+            }
           }
         }
         const float off = m_run == -INFINITY ? 0.f : kHigh - m_run * sc;  // nothing attended yet: all weights are zero
         float sum[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+        bool zeroed = false;
+#pragma unroll 1
+        for (int half = two ? 1 : 0; half >= 0; --half) {
+          if (half == 0 && two) scores(0);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 32 keys at a time
-          uint32_t hi[16], lo[16];
+          for (int c = 0; c < 2; ++c) {  // 32 keys at a time
+            uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
-            fma2(a0, a1, sc, off);
-            a0 = ex2(a0);
-            a1 = ex2(a1);
-            add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
-            hi[k] = pack_h2(a0, a1);
-            if (kTwo) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-              lo[k] = pack_h2(a0 - f.x, a1 - f.y);
+            for (int k = 0; k < 16; ++k) {
+              float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
+              fma2(a0, a1, sc, off);
+              // the special function unit alone would take as long as the MMAs
+              if (!kTwo && (k % 8 == 1 || k % 8 == 4 || k % 8 == 6)) {
+                ex2_fma(a0, a1);
+              } else {
+                a0 = ex2(a0);
+                a1 = ex2(a1);
+              }
+              add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
+              hi[k] = pack_h2(a0, a1);
+              if (kTwo) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                lo[k] = pack_h2(a0 - f.x, a1 - f.y);
+              }
             }
+            tmem_st16(mem + 64 * half + 32 * c, hi);
+            if (kTwo) tmem_st16(mem + 64 * half + 32 * c + 16, lo);
           }
-          tmem_st16(at + 16 * c, hi);
-          if (kTwo) tmem_st16(at + 32 + 16 * c, lo);
+          st_wait();
+          if (half == 1 && !edge) {  // of an edge both wait for the values that are not finite
+            if (j == 0 && tid % 128 == 0) *(volatile int*)&sh.begun[x] = 0;
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.pready[x][1]));
+          }
         }
         l_run += ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
-        st_wait();
-        bool zeroed = false;
         if (edge) {
-          if ((k64 & 1) == 0) {
-            if (!wait_warp(smem_u32(sh.checked + (blk & 1)), (turn >> (4 + (blk & 1))) & 1u)) { failed = true; break; }
-            turn ^= 16u << (blk & 1);
-          }
-          bool first = true;
+          if (!wait_warp(smem_u32(sh.checked + (b & 1)), (turn >> (4 + (b & 1))) & 1u)) { failed = true; break; }
+          turn ^= 16u << (b & 1);
 #pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
+          for (int q = 0; q < 4; ++q) {
 #pragma unroll 1
-            for (uint32_t mask = sh.bad[blk & 1][2 * (k64 & 1) + q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
+            for (uint32_t mask = sh.bad[b & 1][q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
               const int k = 32 * q + __ffs(mask) - 1, key = key0 + k;
-              if (first && k64 > 0) settled();
-              if (first && k64 == 0) {
+              if (j == 0 && !zeroed) {
                 uint32_t z[32];
 #pragma unroll
                 for (int d = 0; d < 32; ++d) z[d] = 0u;
@@ -727,11 +777,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
                 st_wait();
                 zeroed = true;
               }
-              first = false;
               float weight = 0.f;
 #pragma unroll 1
-              for (int c = 0; c <= (kTwo ? 32 : 0); c += 32) {
-                const uint32_t y = tmem_ld1(at + c + k / 2);
+              for (int c = 0; c <= (kTwo ? 16 : 0); c += 16) {
+                const uint32_t y = tmem_ld1(mem + (k & ~31) + c + (k & 31) / 2);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y));
                 weight += k & 1 ? f.y : f.x;
               }
@@ -761,16 +810,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (k64 == 0 && (warp & 3) == 0) *(volatile int*)&sh.begun[x] = zeroed;
-          mbar_arrive(smem_u32(&sh.pready[x][k64 & 1]));
+          if (j == 0 && (warp & 3) == 0 && (edge || !two)) *(volatile int*)&sh.begun[x] = zeroed;
+          if (edge && two) mbar_arrive(smem_u32(&sh.pready[x][1]));
+          mbar_arrive(smem_u32(&sh.pready[x][0]));
         }
       }
-      b += w.blocks;
       if (failed || !wait_warp(smem_u32(sh.odone + x), (turn >> 1) & 1u)) { failed = true; break; }
       turn ^= 2u;
       fence_after();
       // Whole and all that the row attends: its result.  Otherwise what has to be added to others' sums.
       const bool alone = max((len + kPage - 1) / kPage - max(win0 / kPage, w.keys / kPage), 0) == 0;
+      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;  // (the powers on the FMA pipe are never zero)
       const bool result = w.whole && alone;  // (attn_own_kernel writes the zeros of a row that attends nothing)
       const float inv = 1.f / l_run;
       const size_t place = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
@@ -794,9 +844,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
             store8(p, t, head, 32 * c + d, f);
           }
         } else {
-          float4* const dst = reinterpret_cast<float4*>((w.whole ? p.row_o : p.tile_o) + place * kHD + 32 * c);
+          // a cut piece: [32 x 4 dims][256 rows]
+          float4* const dst = reinterpret_cast<float4*>(w.whole ? p.row_o + place * kHD + 32 * c : p.tile_o + ((size_t)w.slot * 32 + 8 * c) * 1024 + 4 * (x * kRows + row));
+          const int step = w.whole ? 1 : 256;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) dst[d] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
+          for (int d = 0; d < 8; ++d) dst[d * step] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
         }
       }
       __syncwarp();
@@ -809,132 +861,64 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 }
 
 // ---- a row's own pages ------------------------------------------------------------------------------------------------------
-// A warp looks after the pages it reads, two on their way.  The query heads of the kv head are the eight columns of every MMA,
-// S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
+// Every warp has pages of its own, of one or several (row, kv head), and keeps two on their way.  The query heads of the kv head are
+// the eight columns of every MMA, S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
 __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const ring = smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u;
   const Groups groups(reinterpret_cast<int*>(smem_raw + kOwnSmem), p.G);
   __shared__ __align__(8) uint64_t full[kRing];
-  __shared__ long long before[kChunks + 1];  // units before chunks of rows
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, cta = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, me = blockIdx.x * kOwnWarps + warp;
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(full + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    p.own_jobs[cta].t = -1;
   }
-  if (!read_groups(p, groups)) {
-    if (cta == 0 && tid == 0) atomicExch(p.status, 6);
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const bool sound_groups = read_groups(p, groups);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");  // for attn_tile_kernel; attn_join_kernel waits for both by waiting for this one
+  if (lane == 0) p.own_jobs[me].t = -1;
+  if (!sound_groups) {
+    if (blockIdx.x == 0 && tid == 0) atomicExch(p.status, 6);
     return;
   }
-  // units of all rows, 32 rows to a warp at a time
-  const int per = 32 * ((p.T + 32 * kChunks - 1) / (32 * kChunks)), chunks = (p.T + per - 1) / per;
-#pragma unroll 4
-  for (int c = warp; c < chunks; c += kOwnWarps) {
-    int n = 0;  // (of 32 rows; of all rows of a chunk at most 2^16 * 2^24)
-    long long sum = 0;
-    for (int t = c * per + lane; t - lane < min((c + 1) * per, p.T); t += 32) {
-      n = t < p.T ? units_of(row_of(p, groups, t)) : 0;
-      sum += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) before[c + 1] = sum;
+  __syncwarp();
+  // rows that attend nothing
+  for (int t0 = 32 * me; t0 < p.T; t0 += 32 * p.own_warps) {
+    const Row r = row_of(p, groups, min(t0 + lane, p.T - 1));
+    for (unsigned empty = __ballot_sync(0xffffffffu, t0 + lane < p.T && r.table_row >= 0 && r.len == 0); empty != 0; empty &= empty - 1)
+      for (int hq = 0; hq < p.Hq; ++hq) store4(p, t0 + __ffs(empty) - 1, hq, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
   }
-  if (tid == 0) before[0] = 0;
-  __syncthreads();
-  if (warp == 0) {
-    long long sum = 0;
-    for (int i = lane; i - lane < chunks; i += 32) {
-      long long x = i < chunks ? before[i + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (i < chunks) before[i + 1] = sum + x;
-      sum += __shfl_sync(0xffffffffu, x, 31);
-    }
-  }
-  __syncthreads();
-  // for attn_join_kernel, and rows that attend nothing: chunks in turn to the CTAs' warps
-  for (int c = cta + warp * (int)gridDim.x; c < chunks; c += kOwnWarps * (int)gridDim.x) {
-    long long sum = before[c];
-    for (int t0 = c * per; t0 < min((c + 1) * per, p.T); t0 += 32) {
-      const int t = t0 + lane;
-      Row r;
-      r.table_row = -1;
-      if (t < p.T) r = row_of(p, groups, t);
-      if (t < p.T && t >= groups.first[0] && t < groups.first[p.G] && p.rows && __ldg(p.rows + t) >= p.table_rows) atomicExch(p.status, 6);
-      const long long n = r.table_row >= 0 ? units_of(r) : 0;
-      long long x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (t < p.T) p.unit_first[t] = sum + x - n;
-      sum += __shfl_sync(0xffffffffu, x, 31);
-      for (unsigned empty = __ballot_sync(0xffffffffu, r.table_row >= 0 && r.len == 0); empty != 0; empty &= empty - 1)
-        for (int hq = 0; hq < p.Hq; ++hq) store4(p, t0 + __ffs(empty) - 1, hq, 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
-    }
-  }
-  const long long all = before[chunks] * p.Hkv, q = share(all, gridDim.x), u0 = min(all, cta * q), u1 = min(all, u0 + q);
-  if (cta == 0 && tid == 0) p.unit_first[p.T] = before[chunks];
-  bool waited = false;  // for attn_tile_kernel
-
-  float (*const sm_o)[8][kHDP] = reinterpret_cast<float (*)[8][kHDP]>(ring);
-  float (*const sm_m)[8] = reinterpret_cast<float (*)[8]>(ring + sizeof(float) * kOwnWarps * 8 * kHDP);
-  float (*const sm_l)[8] = sm_m + kOwnWarps;
-  const uint32_t slots = smem_u32(ring) + (uint32_t)(warp * kDepth) * kSlotBytes, bars = smem_u32(full + warp * kDepth);
+  const long long all = p.unit_first[p.T] * p.Hkv, q = own_share(p), u0 = min(all, me * q), u1 = min(all, u0 + q);
+  unsigned char* const slot0 = ring + (size_t)(warp * kDepth) * kSlotBytes;
+  const uint32_t slots = smem_u32(slot0), bars = smem_u32(full + warp * kDepth);
+  float (*const sm_o)[kHDP] = reinterpret_cast<float (*)[kHDP]>(slot0);  // the warp's sums, when its slots are free
   const int krow = lane & 15, kc = lane >> 4, vrow = 16 + (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
   const float sc = p.scale * kLog2e;
   int slot = 0;
   uint32_t ph = 0;
   bool failed = false;
-  for (long long u = u0; u < u1;) {
-    // the pair of unit u: its rows' thread, then the row among that thread's, 32 at a time
-    int lo = 0, hi = chunks;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before[mid] * p.Hkv <= u) lo = mid;
-      else hi = mid;
+  for (long long u = u0; u < u1 && !failed;) {
+    // the row of unit u: unit_first[t] Hkv <= u < unit_first[t + 1] Hkv, 32 samples at a time
+    int t = 0;
+    for (int hi = p.T; hi - t > 1;) {
+      const int step = (hi - t + 31) / 32, at = min(t + (lane + 1) * step, hi);
+      const unsigned beyond = __ballot_sync(0xffffffffu, p.unit_first[at] * p.Hkv > u);  // (the last one is)
+      const int k = __ffs(beyond) - 1;
+      hi = min(t + (k + 1) * step, hi);
+      t += k * step;
     }
-    int t = lo * per;
-    long long at = before[lo] * p.Hkv;  // units before row t
-    Row row;
-    for (;; t += 32) {
-      const bool there = t + lane < min((lo + 1) * per, p.T);
-      long long n = there ? units_of(row_of(p, groups, t + lane)) : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += y;
-      }
-      const unsigned beyond = __ballot_sync(0xffffffffu, at + n * p.Hkv > u);
-      if (beyond != 0) {
-        const int k = __ffs(beyond) - 1;
-        at += (k > 0 ? __shfl_sync(0xffffffffu, n, k - 1) : 0) * p.Hkv;
-        t += k;
-        break;
-      }
-      at += __shfl_sync(0xffffffffu, n, 31) * p.Hkv;
-    }
-    row = row_of(p, groups, t);
-    const int units = units_of(row), h = (int)divided(u - at, units);
-    const long long pair0 = at + (long long)h * units;       // the pair's units: [pair0, pair0 + units)
-    const long long end = min(u1, pair0 + units);
-    const int first = row.page0 + (int)(u - pair0) * kOwnWarps, last = min(row.page0 + row.pages, row.page0 + (int)(end - pair0) * kOwnWarps);
-    const bool begins = u == pair0, ends = end == pair0 + units;
+    const Row row = row_of(p, groups, t);
+    const long long at = p.unit_first[t] * p.Hkv;
+    const int h = (int)divided(u - at, row.pages);
+    const long long pair0 = at + (long long)h * row.pages;  // the pair's units: its pages
+    const long long end = min(u1, pair0 + row.pages);
+    const int first = row.page0 + (int)(u - pair0), nw = (int)(end - u);
+    const bool begins = u == pair0, ends = end == pair0 + row.pages;
 
-    // ---- pages first + warp, + kOwnWarps, ...
-    const int nw = last - first > warp ? (last - first - warp + kOwnWarps - 1) / kOwnWarps : 0;
-    const int32_t* const ids = p.table + (size_t)row.table_row * p.max_pages + first + warp;
-    auto page_id = [&](int n) { return n < nw ? ids[n * kOwnWarps] : -1; };
+    const int32_t* const ids = p.table + (size_t)row.table_row * p.max_pages + first;
+    auto page_id = [&](int n) { return n < nw ? ids[n] : -1; };
     int pid_cur = page_id(lane), pid_next = page_id(32 + lane);
-    auto fetch = [&](int n, int base, int s) {  // page n of the warp; base: the first page that pid_cur holds
+    auto fetch = [&](int n, int base, int s) {  // page n of the piece; base: the first page that pid_cur holds
       const int pj = __shfl_sync(0xffffffffu, n - base < 32 ? pid_cur : pid_next, n & 31);
       if (lane == 0) {
         if ((unsigned)pj >= (unsigned)p.pool_pages) {  // malformed page table: record, hand over an empty slot
@@ -946,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
         }
       }
     };
-    for (int n = 0; n < kDepth && n < nw && !failed; ++n) fetch(n, 0, (slot + n) % kDepth);
+    for (int n = 0; n < kDepth && n < nw; ++n) fetch(n, 0, (slot + n) % kDepth);
     uint32_t qb[8][2];  // column g = query head h * grp + g (zero columns from grp on)
 #pragma unroll
     for (int j = 0; j < 8; ++j) qb[j][0] = qb[j][1] = 0u;
@@ -983,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
           mma16816(sa[j & 1], ka, qb[j][0], qb[j][1]);
         }
         // log2 domain; lane: tokens g (i < 2) and g + 8, heads 2 t4 and 2 t4 + 1
-        const int tok0 = (first + warp + kOwnWarps * n) * kPage;
+        const int tok0 = (first + n) * kPage;
         const bool edge = tok0 + kPage > row.len || tok0 < row.win0;
         float sv[4];
 #pragma unroll
@@ -1054,54 +1038,34 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
       if (n + kDepth < nw && !failed) fetch(n + kDepth, n & ~31, slot);
       if (++slot == kDepth) { slot = 0; ph ^= 1u; }
     }
-    if (failed) grace();  // copies on their way land before their place is used
+    if (failed) break;
 
-    // ---- the warps' sums: the ring becomes their place ----
-    __syncthreads();
+    // ---- the piece's sums, a head's together: the slots are free
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int o2 = 4; o2 <= 16; o2 <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], o2);
-      const int hh = 2 * t4 + i;
-      if (hh < p.grp) {
-        if (g == 0) {
-          sm_m[warp][hh] = m_run[i];
-          sm_l[warp][hh] = l_run[i];
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sm_o[warp][hh][16 * j + g] = o[j][i];
-          sm_o[warp][hh][16 * j + 8 + g] = o[j][2 + i];
-        }
+      for (int j = 0; j < 8; ++j) {
+        sm_o[2 * t4 + i][16 * j + g] = o[j][i];
+        sm_o[2 * t4 + i][16 * j + 8 + g] = o[j][2 + i];
       }
     }
-    __syncthreads();
+    __syncwarp();
     const bool whole = begins && ends;
-    if (!waited) asm volatile("griddepcontrol.wait;\n" ::: "memory");  // what attn_tile_kernel found is there
-    waited = true;
     int c0 = 0, c1 = 0;
     const bool shared = shared_ctas(p, groups, row, t, h, c0, c1);
-    if (begins && !ends && !(shared && c0 != c1) && tid == 0) {  // cut, and no tile's job: attn_join_kernel adds the pieces
-      qeng_own_job& job = p.own_jobs[cta];
+    if (begins && !ends && !(shared && c0 != c1) && lane == 0) {  // cut, and no tile's job: attn_join_kernel adds the pieces
+      qeng_own_job& job = p.own_jobs[me];
       job.t = t;
       job.h = h;
-      job.last = (int)divided(pair0 + units - 1, q);
+      job.last = (int)divided(pair0 + row.pages - 1, q);
       job.shared = shared;
     }
-    for (int hh = warp; hh < p.grp; hh += kOwnWarps) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kOwnWarps; ++w) M = fmaxf(M, sm_m[w][hh]);
-      float L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kOwnWarps; ++w) {
-        const float f = sm_m[w][hh] == -INFINITY ? 0.f : exp2f(sm_m[w][hh] - M);  // a warp without pages
-        const float4 v = *reinterpret_cast<const float4*>(&sm_o[w][hh][4 * lane]);
-        L += sm_l[w][hh] * f;
-        O.x += v.x * f; O.y += v.y * f; O.z += v.z * f; O.w += v.w * f;
-      }
-      M -= kHigh;
+    for (int hh = 0; hh < p.grp; ++hh) {
+      float M = __shfl_sync(0xffffffffu, hh & 1 ? m_run[1] : m_run[0], hh >> 1) - kHigh;
+      float L = __shfl_sync(0xffffffffu, hh & 1 ? l_run[1] : l_run[0], hh >> 1);
+      float4 O = *reinterpret_cast<const float4*>(&sm_o[hh][4 * lane]);
       const int hq = h * p.grp + hh;
       if (whole && !(shared && c0 != c1)) {
         const size_t place = (size_t)t * p.Hq + hq;
@@ -1111,59 +1075,89 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
       } else {  // whole: a tile's job adds it to the pieces of the shared pages
         float* const o_at = whole ? p.row_o : p.cut_o;
         float* const ml_at = whole ? p.row_ml : p.cut_ml;
-        const size_t place = whole ? (size_t)t * p.Hq + hq : (size_t)(2 * cta + (begins ? 1 : 0)) * 8 + hh;
+        const size_t place = whole ? (size_t)t * p.Hq + hq : (size_t)(2 * me + (begins ? 1 : 0)) * 8 + hh;
         reinterpret_cast<float4*>(o_at + place * kHD)[lane] = O;
         if (lane == 0) reinterpret_cast<float2*>(ml_at)[place] = make_float2(M, L);
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the ring is written by copies again
-    __syncthreads();
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the slots are written by copies again
+    __syncwarp();
     u = end;
   }
-  if (!waited) asm volatile("griddepcontrol.wait;\n" ::: "memory");  // attn_join_kernel waits for both by waiting for this one
-  if (__syncthreads_or(failed) && tid == 0) atomicExch(p.status, 4);
+  if (failed) {
+    if (lane == 0) atomicExch(p.status, 4);
+    grace();
+  }
 }
 
-// ---- what was cut between CTAs: a CTA of attn_tile_kernel left a job for the double tile (and kv head) that it ends with, a CTA of
+// ---- what was cut: a CTA of attn_tile_kernel left a job for the double tile (and kv head) that it ends with, a warp of
 // attn_own_kernel for its last (row, kv head).  A tile's job also takes its rows' own sums, cut or whole.
-constexpr int kJoinWarps = 8, kJoinParts = 16;  // CTAs to a tile's job
+constexpr int kJoinWarps = 8, kJoinParts = 16;  // CTAs to a tile's job: a warp has eight of its 256 rows and a quarter of their dims
 
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_shared_attn p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const long long all = p.unit_first[p.T] * p.Hkv, q = share(all, p.own_ctas);
   if (blockIdx.x < p.tile_ctas * kJoinParts) {
-    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts;
+    // Lane: row lane % 8 of the warp's eight, dims 32 (warp % 4) + 4 (lane / 8) and + 16.
+    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts * kJoinWarps + warp, c0 = 8 * (part & 3) + (lane >> 3);
     const qeng_tile_job job = p.tile_jobs[cta];
-    for (int r = part * kJoinWarps + warp; r < job.rows; r += kJoinParts * kJoinWarps) {
-      const int i = r / p.grp, hh = r - i * p.grp, t = job.t0 + i, hq = job.h * p.grp + hh;
-      if (table_row_of(p, t) < 0 || len_of(p, t) == 0) continue;
+    const int r = (part >> 2) * 8 + (lane & 7), x = r >> 7, i = (r & 127) / p.grp, hh = (r & 127) - i * p.grp, at = x * p.tokens + i;
+    if (i >= p.tokens || at >= job.tokens) return;
+    const int t = job.t0 + at, hq = job.h * p.grp + hh;
+    if (table_row_of(p, t) < 0 || len_of(p, t) == 0) return;
+    const float2* const tile_ml = reinterpret_cast<const float2*>(p.tile_ml) + r;
+    const float4* const tile_o = reinterpret_cast<const float4*>(p.tile_o) + r;
+    const auto slot = [&](int c) { return (size_t)(2 * c + (c == cta ? 1 : 0)); };  // the first CTA ends with it, the others begin with it
+    float M = -INFINITY;
+#pragma unroll 8
+    for (int c = cta; c <= job.last; ++c) M = fmaxf(M, tile_ml[slot(c) * 256].x);
+    const size_t place = (size_t)t * p.Hq + hq;
+    const long long u = p.unit_first[t], units = p.unit_first[t + 1] - u;
+    int e0 = 0, e1 = -1;  // warps with pieces of the row's own pages
+    if (units > 0) {
+      const long long q = own_share(p), y = u * p.Hkv + job.h * units;
+      e0 = (int)divided(y, q);
+      e1 = (int)divided(y + units - 1, q);
+    }
+    const auto own = [&](int e) { return e0 == e1 ? place : (size_t)(2 * e + (e == e0 ? 1 : 0)) * 8 + hh; };
+    const float2* const own_ml = reinterpret_cast<const float2*>(e0 == e1 ? p.row_ml : p.cut_ml);
+    const float4* const own_o = reinterpret_cast<const float4*>(e0 == e1 ? p.row_o : p.cut_o);
+    for (int e = e0; e <= e1; ++e) M = fmaxf(M, own_ml[own(e)].x);
+    float L = 0.f;
+    float4 O[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    // (m, l) = (-inf, NaN): scores of NaN alone; (-inf, 0): nothing attended, or scores of minus infinity alone
+    const auto add = [&](float2 ml, const float4* o, int step) {
+      const bool any = ml.x != -INFINITY;
+      const float f = any ? exp2f(ml.x - M) : 0.f;
+      L += any ? ml.y * f : ml.y;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (any) v = o[(c0 + 4 * k) * step];
+        O[k].x = fmaf(v.x, f, O[k].x); O[k].y = fmaf(v.y, f, O[k].y); O[k].z = fmaf(v.z, f, O[k].z); O[k].w = fmaf(v.w, f, O[k].w);
+      }
+    };
+#pragma unroll 8
+    for (int c = cta; c <= job.last; ++c) add(tile_ml[slot(c) * 256], tile_o + slot(c) * 8192, 256);
+    for (int e = e0; e <= e1; ++e) add(own_ml[own(e)], own_o + own(e) * 32, 1);
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) store4(p, t, hq, 4 * c0 + 16 * k, make_float4(O[k].x * inv, O[k].y * inv, O[k].z * inv, O[k].w * inv));
+  } else {
+    const int me = (blockIdx.x - p.tile_ctas * kJoinParts) * kJoinWarps + warp;
+    if (me >= p.own_warps) return;
+    const qeng_own_job job = p.own_jobs[me];
+    if (job.t < 0) return;
+    for (int hh = 0; hh < p.grp; ++hh) {
       float M = -INFINITY, L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-      add_pieces(lane, cta, job.last, p.tile_o, p.tile_ml, 256, i / p.tokens * 128 + i % p.tokens * p.grp + hh, M, L, O);
-      const long long u = p.unit_first[t], units = p.unit_first[t + 1] - u;
-      if (units > 0) {
-        const long long x = u * p.Hkv + job.h * units;
-        const int d0 = (int)divided(x, q), d1 = (int)divided(x + units - 1, q);
-        const size_t place = (size_t)t * p.Hq + hq;
-        if (d0 == d1) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
-        else add_pieces(lane, d0, d1, p.cut_o, p.cut_ml, 8, hh, M, L, O);
-      }
+      add_pieces(lane, me, job.last, p.cut_o, p.cut_ml, 8, hh, M, L, O);
+      const int hq = job.h * p.grp + hh;
+      const size_t place = (size_t)job.t * p.Hq + hq;
+      if (job.shared) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
       const float inv = 1.f / L;
-      store4(p, t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
+      store4(p, job.t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
     }
-  } else {
-    const int cta = blockIdx.x - p.tile_ctas * kJoinParts;
-    const qeng_own_job job = p.own_jobs[cta];
-    if (job.t < 0 || warp >= p.grp) return;
-    float M = -INFINITY, L = 0.f;
-    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    add_pieces(lane, cta, job.last, p.cut_o, p.cut_ml, 8, warp, M, L, O);
-    const int hq = job.h * p.grp + warp;
-    const size_t place = (size_t)job.t * p.Hq + hq;
-    if (job.shared) add_sums(lane, lane == 0, reinterpret_cast<const float2*>(p.row_ml) + place, p.row_o + place * kHD, M, L, O);
-    const float inv = 1.f / L;
-    store4(p, job.t, hq, 4 * lane, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv));
   }
 }
 
@@ -1222,7 +1216,7 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   p.pool = pool->data; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)pool->kv_heads; p.grp = grp; p.tokens = tokens; p.G = (int)G; p.pool_pages = (int)pool->pages;
   p.window = window; p.softcap = softcap;
   p.scale = scale > 0.f ? scale : 1e-30f;  // nothing, but a masked score (minus infinity) stays what it is
-  p.own_ctas = 3 * ctx->sm_count;
+  p.own_warps = 3 * ctx->sm_count * kOwnWarps;
   p.tile_ctas = ctx->sm_count;
   CUtensorMap map, tile_map, q_map;
   int32_t rc = qeng_kv_map(ctx, pool->data, pool->pages * pool->kv_heads * 32, &map);
@@ -1231,9 +1225,9 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   if (rc != QENG_OK) return rc;
   qeng_scratch* sc = qeng_scratch_for(ctx, st);
   // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml, jobs
-  const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_ctas * 8;
+  const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_warps * 8;
   const size_t need[10] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
-                           p.tile_ctas * sizeof(qeng_tile_job), p.own_ctas * sizeof(qeng_own_job)};
+                           p.tile_ctas * sizeof(qeng_tile_job), p.own_warps * sizeof(qeng_own_job)};
   size_t at[11] = {0};
   for (int i = 0; i < 10; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
   rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[10]);
@@ -1260,11 +1254,11 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = ctx->pdl ? 1 : 0;
-  cfg.gridDim = dim3((unsigned)p.own_ctas);
+  cfg.gridDim = dim3((unsigned)(p.own_warps / kOwnWarps));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kOwnSmem + groups_bytes(G);
   QENG_CUDA(ctx, cudaLaunchKernelEx(&cfg, attn_own_kernel, p, map));
-  cfg.gridDim = dim3((unsigned)(p.tile_ctas * kJoinParts + p.own_ctas));
+  cfg.gridDim = dim3((unsigned)(p.tile_ctas * kJoinParts + (p.own_warps + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   QENG_CUDA(ctx, cudaLaunchKernelEx(&cfg, attn_join_kernel, p));

@@ -6,11 +6,11 @@
 
 constexpr int kSharedGroups = 1024;  // groups of rows in a call
 constexpr int kSharedTiles = 4096;   // and double tiles of them
-constexpr int kOwnWarps = 4;         // of a CTA that reads rows' own pages, and pages of a unit of its work
+constexpr int kOwnWarps = 4;         // of a CTA that reads rows' own pages
 
-// What CTAs leave for attn_join_kernel to add up: `last` is the last CTA that has a piece.
+// What CTAs (or warps) leave for attn_join_kernel to add up: `last` is the last one that has a piece.
 struct qeng_tile_job {
-  int t0, rows, h, last;  // rows of (token, head) of the double tile; none: no job
+  int t0, tokens, h, last;  // tokens of the double tile; none: no job
 };
 struct qeng_own_job {
   int t, h, last, shared;  // t < 0: no job; shared: the row's shared part is in row_o
@@ -26,19 +26,19 @@ struct qeng_shared_attn {
   void* out;
   int32_t* status;
   long long ldq, ldo, max_pages, table_rows;
-  int out_dtype, T, Hq, Hkv, grp, tokens, G, pool_pages, window, own_ctas, tile_ctas;  // tokens: of a tile, 128 / grp
+  int out_dtype, T, Hq, Hkv, grp, tokens, G, pool_pages, window, own_warps, tile_ctas;  // tokens: of a tile, 128 / grp
   float scale, softcap;
   // Working memory: sums that are not a row's whole result, each with (m, l): the sum is of 2^(x - m) v, l of 2^(x - m).
   //
   // The shared pages of a group are worked on by double tiles: 2 * tokens rows, one kv head, all keys that any of them attends, by blocks
   // of 128.  The CTAs of attn_tile_kernel divide all blocks evenly (in the order of double tiles, kv heads,
   // keys), so that a CTA has whole ones but for the first and the last.  The pages that a row has to itself are divided the same way
-  // among the CTAs of attn_own_kernel, in units of four pages.
+  // among the warps of attn_own_kernel.
   int* tile_first;             // [double tiles + 1] blocks (of one kv head) before a double tile
-  float *tile_o, *tile_ml;     // cut between CTAs: [2 tile_ctas][256][128], [..][2]: of what a CTA begins with, of what it ends with
+  float *tile_o, *tile_ml;     // cut between CTAs: [2 tile_ctas][32 x 4 dims][256], [..][256][2]: of what a CTA begins with, of what it ends with
   float *row_o, *row_ml;       // [T][Hq][128], [..][2]: the shared part of a row that has pages to itself, whole; or, where that is cut, the row's own, whole
-  long long* unit_first;       // [T + 1] units (of one kv head) before a row
+  long long* unit_first;       // [T + 1] own pages of the rows before a row
   qeng_tile_job* tile_jobs;    // [tile_ctas]
-  qeng_own_job* own_jobs;      // [own_ctas]
-  float *cut_o, *cut_ml;       // cut between CTAs: [2 own_ctas][8][128], [..][2]
+  qeng_own_job* own_jobs;      // [own_warps]
+  float *cut_o, *cut_ml;       // cut between warps: [2 own_warps][8][128], [..][2]
 };
