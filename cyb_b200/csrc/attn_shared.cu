@@ -24,10 +24,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 // The largest weight of a row is 2^kHigh and more: the smallest that a f16 number holds at full precision is then 2^-21 of it.
 constexpr float kHigh = 7.f;
 
-// K and V of one (page, kv head): 32 rows as two halves of 64 dims, 128-byte swizzled
+// K and V of one (page, kv head): 32 rows as two halves of 64 dims, 128-byte swizzled; nobody else reads it
 __device__ __forceinline__ void page_g2s(uint32_t dst, const CUtensorMap* map, int row, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst), "l"(map), "r"(0),
-               "r"(row), "r"(0), "r"(bar)
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0;\n" : "=l"(policy));
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;\n" ::"r"(dst), "l"(map),
+               "r"(0), "r"(row), "r"(0), "r"(bar), "l"(policy)
                : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -160,9 +162,11 @@ __device__ __forceinline__ long long divided(long long x, long long q) {  // of 
   return ((unsigned long long)(x | q) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)q) : x / q;
 }
 __device__ __forceinline__ long long share(long long all, int n, int least = 1) { return max(divided(all + n - 1, n), (long long)least); }
-constexpr int kLeast = 4;  // pages of a warp of attn_own_kernel at least: cutting a pair costs more than reading that many
+// Work of attn_own_kernel: a (row, kv head) counts kStart pages more than it has, which is what its start and end cost (4 to 5 us, a
+// page 1 us); a warp has kLeast at least, as cutting a pair costs, too.
+constexpr int kStart = 4, kLeast = 10;
+__device__ __forceinline__ int units_of(const Row& r) { return r.pages > 0 ? r.pages + kStart : 0; }
 __device__ __forceinline__ long long own_share(const qeng_shared_attn& p) { return share(p.unit_first[p.T] * p.Hkv, p.own_warps, kLeast); }
-
 // Adds up to 32 sums of one (row, head) to a running (M, L, O): lane i has the i-th, if any; its (m, l) and the place of its 128 values.
 // The lanes' pairs are loaded together and so are the values, four dims a lane.
 __device__ __forceinline__ void add_sums(int lane, bool have, const float2* ml_at, const float* o_at, float& M, float& L, float4& O) {
@@ -287,7 +291,7 @@ __device__ __forceinline__ void count_units(const qeng_shared_attn& p, const Gro
     const int t = t0 + threadIdx.x;
     long long n = 0;
     if (t < p.T) {
-      n = row_of(p, g, t).pages;
+      n = units_of(row_of(p, g, t));
       if (p.rows && t >= g.first[0] && t < g.first[p.G] && __ldg(p.rows + t) >= p.table_rows) atomicExch(p.status, 6);
     }
     long long x = n;
@@ -734,13 +738,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
             for (int k = 0; k < 16; ++k) {
               float &a0 = s[32 * c + 2 * k], &a1 = s[32 * c + 2 * k + 1];
               fma2(a0, a1, sc, off);
-              // the special function unit alone would take as long as the MMAs
-              if (!kTwo && (k % 8 == 1 || k % 8 == 4 || k % 8 == 6)) {
-                ex2_fma(a0, a1);
-              } else {
-                a0 = ex2(a0);
-                a1 = ex2(a1);
-              }
+              a0 = ex2(a0);
+              a1 = ex2(a1);
               add2(sum[2 * (k & 3)], sum[2 * (k & 3) + 1], a0, a1);
               hi[k] = pack_h2(a0, a1);
               if (kTwo) {
@@ -820,7 +819,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       fence_after();
       // Whole and all that the row attends: its result.  Otherwise what has to be added to others' sums.
       const bool alone = max((len + kPage - 1) / kPage - max(win0 / kPage, w.keys / kPage), 0) == 0;
-      if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;  // (the powers on the FMA pipe are never zero)
       const bool result = w.whole && alone;  // (attn_own_kernel writes the zeros of a row that attends nothing)
       const float inv = 1.f / l_run;
       const size_t place = w.whole ? (size_t)t * p.Hq + head : (size_t)w.slot * 256 + x * kRows + row;
@@ -834,7 +832,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         uint32_t o[32];
         __syncwarp();
         tmem_ld32(mem + kO + 32 * c, o);
-        if (!some) continue;
+        if (!live || (result && !some)) continue;
         if (result) {
 #pragma unroll
           for (int d = 0; d < 32; d += 8) {
@@ -848,7 +846,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           float4* const dst = reinterpret_cast<float4*>(w.whole ? p.row_o + place * kHD + 32 * c : p.tile_o + ((size_t)w.slot * 32 + 8 * c) * 1024 + 4 * (x * kRows + row));
           const int step = w.whole ? 1 : 256;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) dst[d * step] = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
+          for (int d = 0; d < 8; ++d) {
+            const float4 v = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
+            dst[d * step] = some ? v : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
         }
       }
       __syncwarp();
@@ -897,23 +898,34 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
   int slot = 0;
   uint32_t ph = 0;
   bool failed = false;
+  int t = -1, h = 0;
+  long long pair0 = 0;  // units before the pair
+  Row row;
   for (long long u = u0; u < u1 && !failed;) {
-    // the row of unit u: unit_first[t] Hkv <= u < unit_first[t + 1] Hkv, 32 samples at a time
-    int t = 0;
-    for (int hi = p.T; hi - t > 1;) {
-      const int step = (hi - t + 31) / 32, at = min(t + (lane + 1) * step, hi);
-      const unsigned beyond = __ballot_sync(0xffffffffu, p.unit_first[at] * p.Hkv > u);  // (the last one is)
-      const int k = __ffs(beyond) - 1;
-      hi = min(t + (k + 1) * step, hi);
-      t += k * step;
+    if (t >= 0 && h + 1 < p.Hkv) {  // the last pair is done
+      ++h;
+    } else {
+      // the row of unit u: unit_first[t] Hkv <= u < unit_first[t + 1] Hkv, 32 samples at a time
+      t = 0;
+      for (int hi = p.T; hi - t > 1;) {
+        const int step = (hi - t + 31) / 32, at = min(t + (lane + 1) * step, hi);
+        const unsigned beyond = __ballot_sync(0xffffffffu, p.unit_first[at] * p.Hkv > u);  // (the last one is)
+        const int k = __ffs(beyond) - 1;
+        hi = min(t + (k + 1) * step, hi);
+        t += k * step;
+      }
+      row = row_of(p, groups, t);
+      const long long at = p.unit_first[t] * p.Hkv;
+      h = (int)divided(u - at, units_of(row));
+      pair0 = at + (long long)h * units_of(row);
     }
-    const Row row = row_of(p, groups, t);
-    const long long at = p.unit_first[t] * p.Hkv;
-    const int h = (int)divided(u - at, row.pages);
-    const long long pair0 = at + (long long)h * row.pages;  // the pair's units: its pages
-    const long long end = min(u1, pair0 + row.pages);
-    const int first = row.page0 + (int)(u - pair0), nw = (int)(end - u);
-    const bool begins = u == pair0, ends = end == pair0 + row.pages;
+    const long long end = min(u1, pair0 + units_of(row));
+    const int past = max((int)(u - pair0) - kStart, 0), nw = (int)(end - pair0) - kStart - past, first = row.page0 + past;
+    const bool begins = past == 0, ends = end == pair0 + units_of(row);
+    if (nw <= 0) {  // what a start costs, and no page
+      u = end;
+      continue;
+    }
 
     const int32_t* const ids = p.table + (size_t)row.table_row * p.max_pages + first;
     auto page_id = [&](int n) { return n < nw ? ids[n] : -1; };
@@ -1059,7 +1071,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
       qeng_own_job& job = p.own_jobs[me];
       job.t = t;
       job.h = h;
-      job.last = (int)divided(pair0 + row.pages - 1, q);
+      job.last = (int)divided(pair0 + units_of(row) - 1, q);
       job.shared = shared;
     }
     for (int hh = 0; hh < p.grp; ++hh) {
@@ -1083,6 +1095,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the slots are written by copies again
     __syncwarp();
     u = end;
+    pair0 = end;
   }
   if (failed) {
     if (lane == 0) atomicExch(p.status, 4);
@@ -1098,51 +1111,89 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_s
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   if (blockIdx.x < p.tile_ctas * kJoinParts) {
-    // Lane: row lane % 8 of the warp's eight, dims 32 (warp % 4) + 4 (lane / 8) and + 16.
-    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts * kJoinWarps + warp, c0 = 8 * (part & 3) + (lane >> 3);
+    // Lane: row lane % 8 of the warp's eight; for the weights every fourth piece, for the values dims 32 (warp % 4) + 4 (lane / 8) + 16 k.
+    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts * kJoinWarps + warp, four = lane >> 3, c0 = 8 * (part & 3) + four;
     const qeng_tile_job job = p.tile_jobs[cta];
     const int r = (part >> 2) * 8 + (lane & 7), x = r >> 7, i = (r & 127) / p.grp, hh = (r & 127) - i * p.grp, at = x * p.tokens + i;
-    if (i >= p.tokens || at >= job.tokens) return;
-    const int t = job.t0 + at, hq = job.h * p.grp + hh;
-    if (table_row_of(p, t) < 0 || len_of(p, t) == 0) return;
-    const float2* const tile_ml = reinterpret_cast<const float2*>(p.tile_ml) + r;
-    const float4* const tile_o = reinterpret_cast<const float4*>(p.tile_o) + r;
-    const auto slot = [&](int c) { return (size_t)(2 * c + (c == cta ? 1 : 0)); };  // the first CTA ends with it, the others begin with it
-    float M = -INFINITY;
-#pragma unroll 8
-    for (int c = cta; c <= job.last; ++c) M = fmaxf(M, tile_ml[slot(c) * 256].x);
-    const size_t place = (size_t)t * p.Hq + hq;
-    const long long u = p.unit_first[t], units = p.unit_first[t + 1] - u;
-    int e0 = 0, e1 = -1;  // warps with pieces of the row's own pages
+    const bool mine = i < p.tokens && at < job.tokens;
+    if (!__any_sync(0xffffffffu, mine)) return;
+    const int t = mine ? job.t0 + at : job.t0, hq = job.h * p.grp + (mine ? hh : 0);
+    const long long u = p.unit_first[t], units = p.unit_first[t + 1] - u, q = own_share(p);
+    const bool live = mine && table_row_of(p, t) >= 0 && len_of(p, t) > 0;
+    int e0 = 0, own = 0;  // warps with pieces of the row's own pages
     if (units > 0) {
-      const long long q = own_share(p), y = u * p.Hkv + job.h * units;
-      e0 = (int)divided(y, q);
-      e1 = (int)divided(y + units - 1, q);
+      const long long y = u * p.Hkv + job.h * units;
+      e0 = (int)divided(y + kStart, q);
+      own = (int)divided(y + units - 1, q) - e0 + 1;
     }
-    const auto own = [&](int e) { return e0 == e1 ? place : (size_t)(2 * e + (e == e0 ? 1 : 0)) * 8 + hh; };
-    const float2* const own_ml = reinterpret_cast<const float2*>(e0 == e1 ? p.row_ml : p.cut_ml);
-    const float4* const own_o = reinterpret_cast<const float4*>(e0 == e1 ? p.row_o : p.cut_o);
-    for (int e = e0; e <= e1; ++e) M = fmaxf(M, own_ml[own(e)].x);
+    const int shared = job.last - cta + 1;  // pieces of the shared pages, two at least
+    const size_t place = (size_t)t * p.Hq + hq;
+    // The first CTA (or warp) ends with what is cut, the others begin with it: the first piece, then those of every second slot.
+    struct Pieces {
+      const float2* ml;
+      const float4* o;
+      int ml_step, o_step;
+    };
+    const float2* const tile_ml = reinterpret_cast<const float2*>(p.tile_ml) + r;
+    const float4* const tile_o = reinterpret_cast<const float4*>(p.tile_o) + r + 256 * c0;
+    const float2* const cut_ml = reinterpret_cast<const float2*>(p.cut_ml) + hh;
+    const float4* const cut_o = reinterpret_cast<const float4*>(p.cut_o) + hh * 32 + c0;
+    const Pieces first = {tile_ml + (size_t)(2 * cta + 1) * 256, tile_o + (size_t)(2 * cta + 1) * 8192, 0, 0};
+    const Pieces rest = {tile_ml + (size_t)(2 * cta + 2) * 256, tile_o + (size_t)(2 * cta + 2) * 8192, 512, 16384};
+    const Pieces own_first = own == 1 ? Pieces{reinterpret_cast<const float2*>(p.row_ml) + place, reinterpret_cast<const float4*>(p.row_o) + place * 32 + c0, 0, 0}
+                                      : Pieces{cut_ml + (size_t)(2 * e0 + 1) * 8, cut_o + (size_t)(2 * e0 + 1) * 256, 0, 0};
+    const Pieces own_rest = {cut_ml + (size_t)(2 * e0 + 2) * 8, cut_o + (size_t)(2 * e0 + 2) * 256, 16, 512};
+    float M = first.ml->x;
+    if (own > 0) M = fmaxf(M, own_first.ml->x);
+    const auto most = [&](const Pieces& a, int n) {  // every fourth piece
+#pragma unroll 4
+      for (int k = four; k < n; k += 4) M = fmaxf(M, a.ml[k * a.ml_step].x);
+    };
+    most(rest, shared - 1);
+    most(own_rest, own - 1);
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
     float L = 0.f;
     float4 O[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    // (m, l) = (-inf, NaN): scores of NaN alone; (-inf, 0): nothing attended, or scores of minus infinity alone
-    const auto add = [&](float2 ml, const float4* o, int step) {
+    const auto add = [&](float2 ml, const float4& v, const float4& w) {
+      // (m, l) = (-inf, NaN): scores of NaN alone; (-inf, 0): nothing attended, or scores of minus infinity alone
       const bool any = ml.x != -INFINITY;
-      const float f = any ? exp2f(ml.x - M) : 0.f;
-      L += any ? ml.y * f : ml.y;
+      const float f = any ? ex2(ml.x - M) : 0.f;
+      L = any ? fmaf(ml.y, f, L) : L + ml.y;
+      O[0].x = fmaf(v.x, f, O[0].x); O[0].y = fmaf(v.y, f, O[0].y); O[0].z = fmaf(v.z, f, O[0].z); O[0].w = fmaf(v.w, f, O[0].w);
+      O[1].x = fmaf(w.x, f, O[1].x); O[1].y = fmaf(w.y, f, O[1].y); O[1].z = fmaf(w.z, f, O[1].z); O[1].w = fmaf(w.w, f, O[1].w);
+    };
+    const auto add_all = [&](Pieces a, int n, int four_dims) {  // four pieces at a time, their loads in front
+      for (; n >= 4; n -= 4) {
+        float2 ml[4];
+        float4 v[4], w[4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (any) v = o[(c0 + 4 * k) * step];
-        O[k].x = fmaf(v.x, f, O[k].x); O[k].y = fmaf(v.y, f, O[k].y); O[k].z = fmaf(v.z, f, O[k].z); O[k].w = fmaf(v.w, f, O[k].w);
+        for (int k = 0; k < 4; ++k) {
+          ml[k] = a.ml[k * a.ml_step];
+          v[k] = a.o[k * a.o_step];
+          w[k] = a.o[k * a.o_step + four_dims];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add(ml[k], v[k], w[k]);
+        a.ml += 4 * a.ml_step;
+        a.o += 4 * a.o_step;
+      }
+      for (; n > 0; --n) {
+        add(*a.ml, a.o[0], a.o[four_dims]);
+        a.ml += a.ml_step;
+        a.o += a.o_step;
       }
     };
-#pragma unroll 8
-    for (int c = cta; c <= job.last; ++c) add(tile_ml[slot(c) * 256], tile_o + slot(c) * 8192, 256);
-    for (int e = e0; e <= e1; ++e) add(own_ml[own(e)], own_o + own(e) * 32, 1);
+    add_all(first, 1, 1024);
+    add_all(rest, shared - 1, 1024);
+    if (own > 0) {
+      add_all(own_first, 1, 4);
+      add_all(own_rest, own - 1, 4);
+    }
     const float inv = 1.f / L;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) store4(p, t, hq, 4 * c0 + 16 * k, make_float4(O[k].x * inv, O[k].y * inv, O[k].z * inv, O[k].w * inv));
+    for (int k = 0; k < 2; ++k)
+      if (live) store4(p, t, hq, 4 * c0 + 16 * k, make_float4(O[k].x * inv, O[k].y * inv, O[k].z * inv, O[k].w * inv));
   } else {
     const int me = (blockIdx.x - p.tile_ctas * kJoinParts) * kJoinWarps + warp;
     if (me >= p.own_warps) return;

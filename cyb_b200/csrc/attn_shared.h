@@ -37,7 +37,7 @@ struct qeng_shared_attn {
   int* tile_first;             // [double tiles + 1] blocks (of one kv head) before a double tile
   float *tile_o, *tile_ml;     // cut between CTAs: [2 tile_ctas][32 x 4 dims][256], [..][256][2]: of what a CTA begins with, of what it ends with
   float *row_o, *row_ml;       // [T][Hq][128], [..][2]: the shared part of a row that has pages to itself, whole; or, where that is cut, the row's own, whole
-  long long* unit_first;       // [T + 1] own pages of the rows before a row
+  long long* unit_first;       // [T + 1] units (of one kv head) of the rows before a row: own pages, and what a start costs
   qeng_tile_job* tile_jobs;    // [tile_ctas]
   qeng_own_job* own_jobs;      // [own_warps]
   float *cut_o, *cut_ml;       // cut between warps: [2 own_warps][8][128], [..][2]

@@ -132,30 +132,8 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, float c) {  
       : "+f"(a0), "+f"(a1)
       : "f"(s), "f"(c));
 }
-__device__ __forceinline__ void fma2v(float& a0, float& a1, float s0, float s1, float c0, float c1) {  // a = a * s + c
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n mov.b64 z, {%4, %5};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "+f"(a0), "+f"(a1)
-      : "f"(s0), "f"(s1), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ void horner2(float& a0, float& a1, float f0, float f1, float c) { fma2v(a0, a1, f0, f1, c, c); }  // a = a * f + c
 __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
   asm("{\n .reg .b64 x, y;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
-}
-
-// 2^x of two numbers below 2^7 on the FMA pipe: 2^n 2^f with n = round(x), 2^f by its minimax polynomial of third degree on
-// [-1/2, 1/2] (relative error 7.5e-5 = 2^-13.7, from the exchange algorithm).  Below -126 it gives 2^-126; NaN stays NaN.
-__device__ __forceinline__ void ex2_fma(float& a0, float& a1) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;\nmax.NaN.f32 %1, %1, 0fC2FC0000;\n" : "+f"(a0), "+f"(a1));
-  float n0 = a0, n1 = a1, b0 = 0.0551716685f, b1 = 0.0551716685f;
-  add2(n0, n1, 12582912.f, 12582912.f);  // 1.5 * 2^23: n in the low bits
-  const float s0 = __uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u), s1 = __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u);
-  add2(n0, n1, -12582912.f, -12582912.f);
-  fma2v(n0, n1, -1.f, -1.f, a0, a1);     // f = x - n
-  horner2(b0, b1, n0, n1, 0.242611125f);
-  horner2(b0, b1, n0, n1, 0.693260968f);
-  horner2(b0, b1, n0, n1, 0.999928057f);
-  a0 = b0 * s0;
-  a1 = b1 * s1;
 }
 
 }  // namespace tc

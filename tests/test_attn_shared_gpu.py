@@ -86,12 +86,11 @@ class Batch:
 
 
 def assert_near(got, want, mag):
-    """Half a step of the result's type; weights of 22 bits (f32 results) or 11, these off by 2^-13 before they are rounded (powers
-    of two by a polynomial of relative error 2^-13.7); 2^-14 of every weight for scores: 128 products summed in f32 at magnitudes
-    up to 2^6, in their exponent."""
+    """Half a step of the result's type; weights of 22 bits (f32 results) or 11; 2^-14 of every weight for scores: 128 products
+    summed in f32 at magnitudes up to 2^6, in their exponent."""
     import torch
     step = torch.finfo(got.dtype).eps / 2
-    weights = 2.0 ** -22 if got.dtype == torch.float32 else 2.0 ** -11 + 2.0 ** -13
+    weights = 2.0 ** -22 if got.dtype == torch.float32 else 2.0 ** -11
     d = (got.double() - want).abs()
     bound = step * want.abs() + (weights + 2.0 ** -14) * mag + 1e-30
     assert torch.isfinite(got).all()
