@@ -48,6 +48,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
+__device__ __forceinline__ float capped(float x, float cap2, float cap) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(ex2(x * cap2) + 1.f));
+  return fmaf(-2.f * cap, y, cap);
+}
+
 // address of 16-byte chunk c (0..15) of row r (16..31: V) of a page
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)((c >> 3) * 4096 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -324,13 +331,6 @@ struct TileShared {
   // added, weights ready (of the first, the second 64 keys); V looked through
   uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2][2], checked[2], drained;
 };
-
-// cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
-__device__ __forceinline__ float capped(float x, float cap2, float cap) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(ex2(x * cap2) + 1.f));
-  return fmaf(-2.f * cap, y, cap);
-}
 
 template <bool kTwo>  // weights as two f16 numbers
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ CUtensorMap qmap) {
@@ -692,9 +692,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           }
           if (edge) {
             const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
+            if (__any_sync(0xffffffffu, e < 64)) {
 #pragma unroll
-            for (int k = 0; k < 64; ++k)
-              if (k >= e || k < a) s[k] = -INFINITY;
+              for (int k = 0; k < 64; ++k) s[k] = k < e ? s[k] : -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, a > 0)) {
+#pragma unroll
+              for (int k = 0; k < 64; ++k) s[k] = k >= a ? s[k] : -INFINITY;
+            }
           }
         };
         float mx = -INFINITY;
@@ -894,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
   const uint32_t slots = smem_u32(slot0), bars = smem_u32(full + warp * kDepth);
   float (*const sm_o)[kHDP] = reinterpret_cast<float (*)[kHDP]>(slot0);  // the warp's sums, when its slots are free
   const int krow = lane & 15, kc = lane >> 4, vrow = 16 + (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
-  const float sc = p.scale * kLog2e;
+  const float sc = p.scale * kLog2e, cap2 = 2.f * kLog2e * p.scale / p.softcap, cap = p.softcap * kLog2e;
   int slot = 0;
   uint32_t ph = 0;
   bool failed = false;
@@ -985,8 +990,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x = sa[0][i] + sa[1][i];
-          if (p.softcap > 0.f) x = p.softcap * tanhf(x * p.scale / p.softcap) * kLog2e;
-          else x *= sc;
+          x = p.softcap > 0.f ? capped(x, cap2, cap) : x * sc;
           if (edge) {
             const int tok = tok0 + g + (i >> 1) * 8;
             if (tok >= row.len || tok < row.win0) x = -INFINITY;
@@ -1002,12 +1006,12 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float m_new = fmaxf(m_run[i], mx[i]);
-          alpha[i] = m_new == -INFINITY ? 1.f : exp2f(m_run[i] - m_new);  // scores of minus infinity so far: weights of zero
+          alpha[i] = m_new == -INFINITY ? 1.f : ex2(m_run[i] - m_new);  // scores of minus infinity so far: weights of zero
           m_run[i] = m_new;
           off[i] = m_new == -INFINITY ? 0.f : m_new - kHigh;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sv[i] = exp2f(sv[i] - off[i & 1]);
+        for (int i = 0; i < 4; ++i) sv[i] = ex2(sv[i] - off[i & 1]);
         l_run[0] = l_run[0] * alpha[0] + (sv[0] + sv[2]);
         l_run[1] = l_run[1] * alpha[1] + (sv[1] + sv[3]);
         if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
@@ -1107,7 +1111,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 // attn_own_kernel for its last (row, kv head).  A tile's job also takes its rows' own sums, cut or whole.
 constexpr int kJoinWarps = 8, kJoinParts = 16;  // CTAs to a tile's job: a warp has eight of its 256 rows and a quarter of their dims
 
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_shared_attn p) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const qeng_shared_attn p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   if (blockIdx.x < p.tile_ctas * kJoinParts) {
@@ -1169,9 +1173,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const qeng_s
         float4 v[4], w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          ml[k] = a.ml[k * a.ml_step];
-          v[k] = a.o[k * a.o_step];
-          w[k] = a.o[k * a.o_step + four_dims];
+          ml[k] = __ldcg(a.ml + k * a.ml_step);
+          v[k] = __ldcg(a.o + k * a.o_step);
+          w[k] = __ldcg(a.o + k * a.o_step + four_dims);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) add(ml[k], v[k], w[k]);
