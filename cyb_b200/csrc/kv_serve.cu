@@ -29,6 +29,7 @@ struct PlanParams {
   int32_t *starts, *slots, *pos, *seen, *rows;
   int32_t* status;
   int R, capacity, pages, ctas;
+  bool whole4;  // the tokens' arrays take 16-byte stores
   long long max_pages, ring_size;
 };
 
@@ -50,7 +51,7 @@ __device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], lo
     if (lane == 31) warps[i][warp] = v[i];
   }
   __syncthreads();
-  if (warp < 3) {
+  if (warp < 3) {  // (four warps at least)
     long long x = lane < nw ? warps[warp][lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -67,6 +68,9 @@ __device__ __forceinline__ void scan3(long long (&v)[3], long long (&tot)[3], lo
   }
   __syncthreads();  // `warps` may be written again
 }
+
+// of numbers that are not negative; most fit 32 bits
+__device__ __forceinline__ long long remainder_of(long long x, long long n) { return ((x | n) >> 32) == 0 ? (long long)((uint32_t)x % (uint32_t)n) : x % n; }
 
 // last r in [lo, n) with first[r] <= x (first ascends, first[lo] <= x)
 __device__ __forceinline__ int find_row(const int* first, int lo, int n, int x) {
@@ -151,34 +155,55 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
   __syncthreads();
   if (p.ctas > 1) cluster_arrive();  // this CTA has read lengths and counters
 
-  const long long h0 = head % p.ring_size, t0 = tail % p.ring_size;
+  const long long h0 = remainder_of(head, p.ring_size), t0 = remainder_of(tail, p.ring_size);
   const auto ring_at = [&](long long at, long long i) {
     const long long x = at + i;  // i <= ring_size
     return x >= p.ring_size ? x - p.ring_size : x;
   };
   const int self = cta * nt + tid, all = p.ctas * nt;
-  // tokens, four in a row to a thread
+  // tokens, four in a row to a thread: most of them share a page
   for (int t = 4 * self; t < p.capacity; t += 4 * all) {
-    int r = t < tokens ? find_row(tok, 0, p.R, t) : 0;
+    int slot[4], at[4], n[4], row[4];
+    int r = t < tokens ? find_row(tok, 0, p.R, t) : 0, of = -1, id = -1;  // page `of` of request r
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int u = t + i;
-      if (u >= p.capacity) break;
-      int slot = -1, at = 0, n = 0, row = -1;
+      slot[i] = row[i] = -1;
+      at[i] = n[i] = 0;
       if (u < tokens) {
-        while (tok[r + 1] <= u) ++r;
-        row = r;
-        at = len[r] + (u - tok[r]);
-        n = at + 1;
-        const int old = (len[r] + kPage - 1) / kPage, pg = at / kPage;
-        const int id = pg < old ? p.table[(size_t)r * p.max_pages + pg] : p.ring[ring_at(h0, page[r] + (pg - old))];
-        if ((unsigned)id < (unsigned)p.pages) slot = id * kPage + at % kPage;
-        else atomicExch(p.status, 1);
+        while (tok[r + 1] <= u) {
+          ++r;
+          of = -1;
+        }
+        row[i] = r;
+        at[i] = len[r] + (u - tok[r]);
+        n[i] = at[i] + 1;
+        const int old = (len[r] + kPage - 1) / kPage, pg = at[i] / kPage;
+        if (pg != of) {
+          of = pg;
+          id = pg < old ? p.table[(size_t)r * p.max_pages + pg] : p.ring[ring_at(h0, page[r] + (pg - old))];
+          if ((unsigned)id >= (unsigned)p.pages) {
+            id = -1;
+            atomicExch(p.status, 1);
+          }
+        }
+        if (id >= 0) slot[i] = id * kPage + at[i] % kPage;
       }
-      p.slots[u] = slot;
-      p.pos[u] = at;
-      p.seen[u] = n;
-      p.rows[u] = row;
+    }
+    if (p.whole4) {
+      *reinterpret_cast<int4*>(p.slots + t) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(p.pos + t) = make_int4(at[0], at[1], at[2], at[3]);
+      *reinterpret_cast<int4*>(p.seen + t) = make_int4(n[0], n[1], n[2], n[3]);
+      *reinterpret_cast<int4*>(p.rows + t) = make_int4(row[0], row[1], row[2], row[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < p.capacity) {
+          p.slots[t + i] = slot[i];
+          p.pos[t + i] = at[i];
+          p.seen[t + i] = n[i];
+          p.rows[t + i] = row[i];
+        }
     }
   }
   for (int i = self; i < taken; i += all) {
@@ -230,20 +255,14 @@ struct AppendParams {
   double log2_base;
 };
 
-constexpr int kAppendThreads = 256, kHeadLanes = 16, kAtOnce = 4;  // heads of a lane on their way together
+constexpr int kAppendThreads = 256, kHeadLanes = 16, kAtOnce = 3;  // heads of a lane on their way together
 
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) rope_append_slots_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) rope_append_slots_kernel(const AppendParams p) {
   __shared__ float cs[2][64];
   const int tid = threadIdx.x, l = tid % kHeadLanes, lane_head = tid / kHeadLanes;
   constexpr int kStep = kAppendThreads / kHeadLanes;
   const size_t t = blockIdx.x;
-  const int slot = p.slots[t];
-  if (slot < 0) return;  // padding
-  if (slot >= p.places) {
-    if (tid == 0) atomicExch(p.status, 1);
-    return;
-  }
   const int heads = p.Hq + 2 * p.Hkv;
   const T* const x = static_cast<const T*>(p.x) + t * p.ldx;
   float4 a[kAtOnce], b[kAtOnce];
@@ -257,10 +276,16 @@ __global__ void __launch_bounds__(kAppendThreads) rope_append_slots_kernel(const
       }
     }
   };
-  load(lane_head);
+  load(lane_head);  // on its way while the slot and the position are
+  const int slot = p.slots[t], pos = p.pos[t];
+  if (slot < 0) return;  // padding
+  if (slot >= p.places) {
+    if (tid == 0) atomicExch(p.status, 1);
+    return;
+  }
   if (tid < 64) {
     // whole turns leave the angle in 64 bits: in 32 a position of 10^5 would be off by 10^-3
-    double turns = p.pos[t] * exp2(-(double)tid / 64 * p.log2_base) * 0.15915494309189533577;
+    double turns = pos * exp2(-(double)tid / 64 * p.log2_base) * 0.15915494309189533577;
     turns -= rint(turns);
     float s, c;
     sincospif((float)(2 * turns), &s, &c);
@@ -325,8 +350,13 @@ int32_t qeng_kv_plan(qeng_ctx* ctx, const qeng_kv_pool* pool, int64_t R, const i
   p.lens = lens; p.add = add; p.keep = keep; p.table = page_table; p.ring = ring; p.ends = ends; p.lens_out = lens_out; p.ends_out = ends_out;
   p.starts = starts; p.slots = slots; p.pos = pos; p.seen = seen; p.rows = rows; p.status = ctx->status;
   p.R = (int)R; p.capacity = (int)capacity; p.pages = (int)pool->pages; p.max_pages = max_pages; p.ring_size = ring_size;
+  p.whole4 = capacity % 4 == 0 &&
+             ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(seen) | reinterpret_cast<uintptr_t>(rows)) & 15) == 0;
+  // a thread for every request and four tokens as far as a block has them (barriers of few warps are faster), clusters above
   p.ctas = 1;
   while (p.ctas < 8 && capacity > 4096ll * p.ctas) p.ctas *= 2;
+  int threads = 128;
+  while (threads < kPlanThreads && (threads < R || 4ll * threads < capacity)) threads *= 2;
   const size_t smem = (size_t)(4 * R + 3) * sizeof(int);
   static bool configured_on[64] = {};  // the opt-in shared-memory size is set per device
   bool& configured = configured_on[ctx->device & 63];
@@ -336,7 +366,7 @@ int32_t qeng_kv_plan(qeng_ctx* ctx, const qeng_kv_pool* pool, int64_t R, const i
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.ctas);
-  cfg.blockDim = dim3(kPlanThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];

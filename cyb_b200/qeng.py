@@ -399,7 +399,7 @@ class Context:
         import torch
         n, dev = requests, "cuda:%d" % self.device
         ints = torch.empty(2 * n + 1 + 4 * capacity, dtype=torch.int32, device=dev)
-        starts, lens, slots, pos, seen, rows = ints.split([n + 1, n] + [capacity] * 4)
+        slots, pos, seen, rows, starts, lens = ints.split([capacity] * 4 + [n + 1, n])
         return KVPlan(starts, slots, pos, seen, rows, lens, torch.empty(2, dtype=torch.int64, device=dev))
 
     def kv_plan(self, pool, lens, add, table, ring, ends, capacity, keep=None, out=None):
