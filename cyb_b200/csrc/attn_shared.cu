@@ -171,7 +171,7 @@ __device__ __forceinline__ long long divided(long long x, long long q) {  // of 
 __device__ __forceinline__ long long share(long long all, int n, int least = 1) { return max(divided(all + n - 1, n), (long long)least); }
 // Work of attn_own_kernel: a (row, kv head) counts kStart pages more than it has, which is what its start and end cost (4 to 5 us, a
 // page 1 us); a warp has kLeast at least, as cutting a pair costs, too.
-constexpr int kStart = 4, kLeast = 10;
+constexpr int kStart = 4, kLeast = 6;
 __device__ __forceinline__ int units_of(const Row& r) { return r.pages > 0 ? r.pages + kStart : 0; }
 __device__ __forceinline__ long long own_share(const qeng_shared_attn& p) { return share(p.unit_first[p.T] * p.Hkv, p.own_warps, kLeast); }
 // Adds up to 32 sums of one (row, head) to a running (M, L, O): lane i has the i-th, if any; its (m, l) and the place of its 128 values.
@@ -884,10 +884,23 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
   asm volatile("griddepcontrol.wait;\n" ::: "memory");  // for attn_tile_kernel; attn_join_kernel waits for both by waiting for this one
   if (lane == 0) p.own_jobs[me].t = -1;
   if (!sound_groups) {
-    if (blockIdx.x == 0 && tid == 0) atomicExch(p.status, 6);
+    if (me == 0 && lane == 0) {
+      atomicExch(p.status, 6);
+      p.tile_list[0] = 0;
+    }
     return;
   }
   __syncwarp();
+  if (me == 0) {  // the CTAs of attn_tile_kernel that left a job, and how many in front: attn_join_kernel begins with them
+    int n = 0;
+    for (int c0 = 0; c0 < p.tile_ctas; c0 += 32) {
+      const int c = c0 + lane;
+      const unsigned with = __ballot_sync(0xffffffffu, c < p.tile_ctas && p.tile_jobs[min(c, p.tile_ctas - 1)].tokens > 0);
+      if ((with >> lane) & 1u) p.tile_list[1 + n + __popc(with & ((1u << lane) - 1u))] = c;
+      n += __popc(with);
+    }
+    if (lane == 0) p.tile_list[0] = n;
+  }
   // rows that attend nothing
   for (int t0 = 32 * me; t0 < p.T; t0 += 32 * p.own_warps) {
     const Row r = row_of(p, groups, min(t0 + lane, p.T - 1));
@@ -1116,7 +1129,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const qen
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   if (blockIdx.x < p.tile_ctas * kJoinParts) {
     // Lane: row lane % 8 of the warp's eight; for the weights every fourth piece, for the values dims 32 (warp % 4) + 4 (lane / 8) + 16 k.
-    const int cta = blockIdx.x / kJoinParts, part = blockIdx.x % kJoinParts * kJoinWarps + warp, four = lane >> 3, c0 = 8 * (part & 3) + four;
+    const int index = blockIdx.x / kJoinParts;
+    if (index >= p.tile_list[0]) return;
+    const int cta = p.tile_list[1 + index], part = blockIdx.x % kJoinParts * kJoinWarps + warp, four = lane >> 3, c0 = 8 * (part & 3) + four;
     const qeng_tile_job job = p.tile_jobs[cta];
     const int r = (part >> 2) * 8 + (lane & 7), x = r >> 7, i = (r & 127) / p.grp, hh = (r & 127) - i * p.grp, at = x * p.tokens + i;
     const bool mine = i < p.tokens && at < job.tokens;
@@ -1168,32 +1183,28 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const qen
       O[1].x = fmaf(w.x, f, O[1].x); O[1].y = fmaf(w.y, f, O[1].y); O[1].z = fmaf(w.z, f, O[1].z); O[1].w = fmaf(w.w, f, O[1].w);
     };
     const auto add_all = [&](Pieces a, int n, int four_dims) {  // four pieces at a time, their loads in front
-      for (; n >= 4; n -= 4) {
+      for (; n > 0; n -= 4) {
         float2 ml[4];
         float4 v[4], w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          ml[k] = __ldcg(a.ml + k * a.ml_step);
-          v[k] = __ldcg(a.o + k * a.o_step);
-          w[k] = __ldcg(a.o + k * a.o_step + four_dims);
+          const bool more = k < n;  // (behind the last one: no weight)
+          ml[k] = more ? __ldcg(a.ml) : make_float2(-INFINITY, 0.f);
+          v[k] = more ? __ldcg(a.o) : make_float4(0.f, 0.f, 0.f, 0.f);
+          w[k] = more ? __ldcg(a.o + four_dims) : make_float4(0.f, 0.f, 0.f, 0.f);
+          a.ml += a.ml_step;
+          a.o += a.o_step;
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) add(ml[k], v[k], w[k]);
-        a.ml += 4 * a.ml_step;
-        a.o += 4 * a.o_step;
-      }
-      for (; n > 0; --n) {
-        add(*a.ml, a.o[0], a.o[four_dims]);
-        a.ml += a.ml_step;
-        a.o += a.o_step;
       }
     };
-    add_all(first, 1, 1024);
+    const float2 ml0 = *first.ml, ml1 = *own_first.ml;
+    const float4 v0 = first.o[0], w0 = first.o[1024], v1 = own_first.o[0], w1 = own_first.o[4];
     add_all(rest, shared - 1, 1024);
-    if (own > 0) {
-      add_all(own_first, 1, 4);
-      add_all(own_rest, own - 1, 4);
-    }
+    add_all(own_rest, own - 1, 4);
+    add(ml0, v0, w0);
+    if (own > 0) add(ml1, v1, w1);
     const float inv = 1.f / L;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -1281,11 +1292,12 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   qeng_scratch* sc = qeng_scratch_for(ctx, st);
   // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml, jobs
   const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_warps * 8;
-  const size_t need[10] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
-                           p.tile_ctas * sizeof(qeng_tile_job), p.own_warps * sizeof(qeng_own_job)};
-  size_t at[11] = {0};
-  for (int i = 0; i < 10; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
-  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[10]);
+  const size_t need[11] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
+                           p.tile_ctas * sizeof(qeng_tile_job), p.own_warps * sizeof(qeng_own_job),
+                           (size_t)(1 + p.tile_ctas) * 4};
+  size_t at[12] = {0};
+  for (int i = 0; i < 11; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
+  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[11]);
   if (rc != QENG_OK) return rc;
   unsigned char* const mem = static_cast<unsigned char*>(sc->shared.ptr);
   p.tile_first = reinterpret_cast<int*>(mem);
@@ -1298,6 +1310,7 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   p.cut_ml = reinterpret_cast<float*>(mem + at[7]);
   p.tile_jobs = reinterpret_cast<qeng_tile_job*>(mem + at[8]);
   p.own_jobs = reinterpret_cast<qeng_own_job*>(mem + at[9]);
+  p.tile_list = reinterpret_cast<int*>(mem + at[10]);
   if (out_dtype == QENG_F32) attn_tile_kernel<true><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   else attn_tile_kernel<false><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   QENG_LAUNCH_CHECK(ctx);

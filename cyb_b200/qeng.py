@@ -406,15 +406,16 @@ class Context:
         """Pages and slots for add[r] more tokens of every request, see qeng_kv_plan: the table and the ring are updated, the rest
         comes back as a KVPlan.  `out`: a KVPlan to fill; its lens and ends may be the arguments themselves."""
         import torch
-        n = lens.numel()
-        for t, ty in ((lens, torch.int32), (add, torch.int32), (table, torch.int32), (ring, torch.int32), (ends, torch.int64)):
-            assert t.is_cuda and t.dtype == ty and t.is_contiguous()
-        assert add.numel() == n and ends.numel() == 2 and table.dim() == 2 and table.shape[0] >= n
-        assert keep is None or (keep.is_cuda and keep.dtype == torch.int32 and keep.is_contiguous() and keep.numel() == n)
+        i32, n = torch.int32, lens.numel()
+        for t in (lens, add, table, ring) if keep is None else (lens, add, table, ring, keep):
+            assert t.is_cuda and t.dtype is i32 and t.is_contiguous()
+        assert ends.is_cuda and ends.dtype is torch.int64 and ends.is_contiguous() and ends.numel() == 2
+        rows, width = table.shape
+        assert add.numel() == n and rows >= n and (keep is None or keep.numel() == n)
         if out is None:
             out = self.kv_plan_buffers(n, capacity)
         assert out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
-        rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), table.shape[1],
+        rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), width,
                                ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
                                out.slots.data_ptr(), out.pos.data_ptr(), out.seen.data_ptr(), out.rows.data_ptr(), capacity, _cur_stream())
         if rc:
@@ -426,17 +427,18 @@ class Context:
         heads, rotation, k and v into the pool at `slots`; returns q as float16 [T, Hq, 128].  Rows with a negative slot are left alone
         (those of a new result are then not initialised)."""
         import torch
-        dt = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[qkv.dtype]
-        t, width = qkv.shape
-        hq = width // pool.hd - 2 * pool.kv_heads
-        assert qkv.is_cuda and qkv.stride(1) == 1 and width % pool.hd == 0
-        assert pos.dtype == slots.dtype == torch.int32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == slots.numel() == t
+        (t, width), hd, i32 = qkv.shape, pool.hd, torch.int32
+        hq = width // hd - 2 * pool.kv_heads
+        ld, one = qkv.stride()
+        assert qkv.is_cuda and one == 1 and width % hd == 0
+        assert pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
         if out is None:
-            out = qkv.new_empty((t, hq, pool.hd), dtype=torch.float16)
-        assert out.dtype == torch.float16 and out.shape == (t, hq, pool.hd) and out.stride(2) == 1 and out.stride(1) == pool.hd
-        rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), dt, t, qkv.stride(0) if t > 1 else width, hq,
+            out = qkv.new_empty((t, hq, hd), dtype=torch.float16)
+        ldq, per_head, per_dim = out.stride()
+        assert out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
+        rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), _dtype(qkv), t, ld if t > 1 else width, hq,
                                    None if q_gain is None else _gain(q_gain), None if k_gain is None else _gain(k_gain), eps, pos.data_ptr(),
-                                   slots.data_ptr(), base, out.data_ptr(), out.stride(0) if t > 1 else hq * pool.hd, _cur_stream())
+                                   slots.data_ptr(), base, out.data_ptr(), ldq if t > 1 else hq * hd, _cur_stream())
         if rc:
             self.check(rc)
         return out
@@ -447,26 +449,38 @@ class Context:
         `dtype` (float32, float16 or bfloat16; None: float32); rows in no group, or of table row -1, are left alone (those of a new result
         are then not initialised)."""
         import torch
-        t, hq, hd = q.shape
-        assert q.dtype == torch.float16 and q.stride(2) == 1 and q.stride(1) == hd
+        (t, hq, hd), i32 = q.shape, torch.int32
+        ldq, per_head, per_dim = q.stride()
+        assert q.dtype is torch.float16 and per_dim == 1 and per_head == hd
         for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
-            assert x.is_cuda and x.dtype == torch.int32 and x.is_contiguous()
-        g = group_pages.numel()
-        assert lens.numel() == t and group_first.numel() == g + 1 and table.dim() == 2 and (rows is None or rows.numel() == t)
+            assert x.is_cuda and x.dtype is i32 and x.is_contiguous()
+        (table_rows, width), g = table.shape, group_pages.numel()
+        assert lens.numel() == t and group_first.numel() == g + 1 and (rows is None or rows.numel() == t)
         if out is None:
             out = q.new_empty((t, hq, hd), dtype=dtype or torch.float32)
-        assert out.shape == q.shape and dtype in (None, out.dtype) and out.stride(2) == 1 and out.stride(1) == hd
-        width = hq * hd
-        rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), q.stride(0) if t > 1 else width, table.data_ptr(), table.shape[1], table.shape[0],
+        ldo, per_head, per_dim = out.stride()
+        assert out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
+        rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), ldq if t > 1 else hq * hd, table.data_ptr(), width, table_rows,
                                    None if rows is None else rows.data_ptr(), lens.data_ptr(), t, hq, group_first.data_ptr(), group_pages.data_ptr(), g,
-                                   float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(),
-                                   {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[out.dtype], out.stride(0) if t > 1 else width, _cur_stream())
+                                   float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(), _dtype(out), ldo if t > 1 else hq * hd,
+                                   _cur_stream())
         if rc:
             self.check(rc)
         return out
 
     def decoder(self, **kw):
         return Decoder(self, **kw)
+
+
+_DTYPES = {}
+
+
+def _dtype(t):
+    """QENG_F32 / F16 / BF16 of a tensor."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _DTYPES[t.dtype]
 
 
 def _gain(t):
