@@ -48,13 +48,24 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// cap * tanh: 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
-__device__ __forceinline__ float capped(float x, float cap2, float cap) {
+__device__ __forceinline__ float rcp(float x) {
   float y;
-  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(ex2(x * cap2) + 1.f));
-  return fmaf(-2.f * cap, y, cap);
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
 }
-
+// cap * tanh(y), cap2 x = 2 y log2(e): 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
+__device__ __forceinline__ float capped(float x, float cap2, float cap) { return fmaf(-2.f * cap, rcp(ex2(x * cap2) + 1.f), cap); }
+// The same for f32 results: below 0.6, where scores mostly are and the difference above cancels, y + y^3 P(y^2), P fitted at Chebyshev
+// nodes (relative error 2^-23.6).
+__device__ __forceinline__ float capped_f32(float x, float cap2, float cap) {
+  const float y = x * (cap2 * 0.34657359027997264f), z = y * y;  // ln(2) / 2
+  float p = fmaf(-0.006276387721f, z, 0.02111621387f);
+  p = fmaf(p, z, -0.05387513712f);
+  p = fmaf(p, z, 0.1333292425f);
+  p = fmaf(p, z, -0.3333333135f);
+  const float big = fmaf(-2.f, rcp(ex2(fabsf(x * cap2)) + 1.f), 1.f);
+  return cap * (fabsf(y) < 0.6f ? fmaf(y * z, p, y) : copysignf(big, y));
+}
 // address of 16-byte chunk c (0..15) of row r (16..31: V) of a page
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)((c >> 3) * 4096 + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -245,6 +256,9 @@ constexpr int kTileThreads = (kCheckWarp + kCheckWarps) * 32;
 constexpr size_t kTileSmem = 6 * kTileBytes + 1024;
 // Columns of a tile: scores at 0; the weights of 32 keys take the place of their scores, the second terms 16 columns behind the first.
 constexpr uint32_t kO = 128;
+// The MMAs cut the sums that they add to: 3e-7 of O a block with two terms.  For f32 results O starts anew every kFresh blocks, and what
+// it held is added up in memory (in L2), rounded to nearest.
+constexpr int kFresh = 2;
 constexpr float kGrow = 8.f;   // weights reach 2^(kHigh + kGrow), below the largest f16 number
 
 // Some blocks of a double tile.
@@ -562,7 +576,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
                 }
               }
               fence_after();
-              uint32_t acc = !first || j > 0 || *(volatile int*)&sh.begun[x];
+              uint32_t acc = !first || (kTwo ? j % kFresh != 0 : j > 0) || *(volatile int*)&sh.begun[x];
               const int steps = (left - 64 * half + kPage - 1) / kPage;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -651,6 +665,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
     const uint32_t mem = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)x * 256u;
     const float sc = p.softcap > 0.f ? 1.f : p.scale * kLog2e;
     const float cap2 = 2.f * kLog2e * p.scale / p.softcap, cap = p.softcap * kLog2e;
+    float4* const kept = reinterpret_cast<float4*>(p.kept_o) + (size_t)cta * 8192 + x * kRows + row;  // this lane's; [32 x 4 dims][256 rows] of a CTA
     int b = 0;
     uint32_t turn = 0;  // parities of sdone (bit 0), odone (1) and checked (4 + slot)
     while (const Piece* const piece = next_piece()) {
@@ -673,10 +688,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       // a row that attends none of these keys attends everything, to nobody's use
       const int begin = some ? win0 : 0, end = some ? min(len, w.keys) : 0x7fffffff;
       float m_run = -INFINITY, l_run = 0.f;
+      float scale_kept = 1.f;  // of what `kept` holds, since it was last written
 #pragma unroll 1
       for (int j = 0; j < w.blocks; ++j, ++b) {
         const int key0 = (w.page0 + 8 * j) * kPage;
-        const bool edge = is_edge(w, j);
+        const bool edge = is_edge(w, j), fresh = kTwo ? j % kFresh == 0 : j == 0;
         if (!wait_warp(smem_u32(sh.sdone + x), turn & 1u)) { failed = true; break; }
         turn ^= 1u;
         fence_after();
@@ -688,7 +704,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
           if (p.softcap > 0.f) {
 #pragma unroll
-            for (int k = 0; k < 64; ++k) s[k] = capped(s[k], cap2, cap);
+            for (int k = 0; k < 64; ++k) s[k] = kTwo ? capped_f32(s[k], cap2, cap) : capped(s[k], cap2, cap);
           }
           if (edge) {
             const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
@@ -717,6 +733,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           const float alpha = !moved ? 1.f : m_run == -INFINITY ? 0.f : ex2((m_run - mx) * sc);
           if (moved) m_run = mx;
           l_run *= alpha;
+          scale_kept *= alpha;
           if (j > 0) {  // the values of the block before are in (its scores came behind them), the next wait for this warp
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -727,6 +744,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
               tmem_st32(mem + kO + 32 * c, o);
             }
           }
+        }
+        if (kTwo && fresh && j > 0) {
+          st_wait();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float4 before[8];
+            if (j > kFresh) {
+#pragma unroll
+              for (int d = 0; d < 8; ++d) before[d] = __ldcg(kept + (8 * c + d) * 256);
+            }
+            uint32_t o[32];
+            tmem_ld32(mem + kO + 32 * c, o);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+              float4 v = make_float4(__uint_as_float(o[4 * d]), __uint_as_float(o[4 * d + 1]), __uint_as_float(o[4 * d + 2]), __uint_as_float(o[4 * d + 3]));
+              if (j > kFresh)
+                v = make_float4(fmaf(before[d].x, scale_kept, v.x), fmaf(before[d].y, scale_kept, v.y), fmaf(before[d].z, scale_kept, v.z), fmaf(before[d].w, scale_kept, v.w));
+              __stcg(kept + (8 * c + d) * 256, v);
+            }
+          }
+          scale_kept = 1.f;
         }
         const float off = m_run == -INFINITY ? 0.f : kHigh - m_run * sc;  // nothing attended yet: all weights are zero
         float sum[8];
@@ -757,7 +795,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           }
           st_wait();
           if (half == 1 && !edge) {  // of an edge both wait for the values that are not finite
-            if (j == 0 && tid % 128 == 0) *(volatile int*)&sh.begun[x] = 0;
+            if (fresh && tid % 128 == 0) *(volatile int*)&sh.begun[x] = 0;
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.pready[x][1]));
@@ -772,7 +810,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 #pragma unroll 1
             for (uint32_t mask = sh.bad[b & 1][q]; mask != 0; mask &= mask - 1) {  // the same in all lanes
               const int k = 32 * q + __ffs(mask) - 1, key = key0 + k;
-              if (j == 0 && !zeroed) {
+              if (fresh && !zeroed) {
                 uint32_t z[32];
 #pragma unroll
                 for (int d = 0; d < 32; ++d) z[d] = 0u;
@@ -814,7 +852,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (j == 0 && (warp & 3) == 0 && (edge || !two)) *(volatile int*)&sh.begun[x] = zeroed;
+          if (fresh && (warp & 3) == 0 && (edge || !two)) *(volatile int*)&sh.begun[x] = zeroed;
           if (edge && two) mbar_arrive(smem_u32(&sh.pready[x][1]));
           mbar_arrive(smem_u32(&sh.pready[x][0]));
         }
@@ -837,6 +875,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         uint32_t o[32];
         __syncwarp();
         tmem_ld32(mem + kO + 32 * c, o);
+        if (kTwo && w.blocks > kFresh) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            const float4 v = __ldcg(kept + (8 * c + d) * 256);
+            o[4 * d] = __float_as_uint(fmaf(v.x, scale_kept, __uint_as_float(o[4 * d])));
+            o[4 * d + 1] = __float_as_uint(fmaf(v.y, scale_kept, __uint_as_float(o[4 * d + 1])));
+            o[4 * d + 2] = __float_as_uint(fmaf(v.z, scale_kept, __uint_as_float(o[4 * d + 2])));
+            o[4 * d + 3] = __float_as_uint(fmaf(v.w, scale_kept, __uint_as_float(o[4 * d + 3])));
+          }
+        }
         if (!live || (result && !some)) continue;
         if (result) {
 #pragma unroll
@@ -1003,7 +1051,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float x = sa[0][i] + sa[1][i];
-          x = p.softcap > 0.f ? capped(x, cap2, cap) : x * sc;
+          x = p.softcap > 0.f ? capped_f32(x, cap2, cap) : x * sc;
           if (edge) {
             const int tok = tok0 + g + (i >> 1) * 8;
             if (tok >= row.len || tok < row.win0) x = -INFINITY;
@@ -1059,8 +1107,12 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
             va[0] &= keep[0]; va[1] &= keep[0];
             va[2] &= keep[1]; va[3] &= keep[1];
           }
-          mma16816(o[j], va, hi2[0], hi2[1]);
-          mma16816(o[j], va, lo2[0], lo2[1]);
+          // a page's values by themselves: the MMAs cut what they add to, which would show after some dozens
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816(d, va, hi2[0], hi2[1]);
+          mma16816(d, va, lo2[0], lo2[1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][i] += d[i];
         }
       }
       __syncwarp();
@@ -1292,12 +1344,12 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   qeng_scratch* sc = qeng_scratch_for(ctx, st);
   // tile_first, tile_o, tile_ml, row_o, row_ml, unit_first, cut_o, cut_ml, jobs
   const size_t cut = (size_t)2 * p.tile_ctas * 256, rows_heads = (size_t)T * Hq, own = (size_t)2 * p.own_warps * 8;
-  const size_t need[11] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
+  const size_t need[12] = {(size_t)(tiles + 1) * 4, cut * kHD * 4, cut * 8, rows_heads * kHD * 4, rows_heads * 8, ((size_t)T + 1) * 8, own * kHD * 4, own * 8,
                            p.tile_ctas * sizeof(qeng_tile_job), p.own_warps * sizeof(qeng_own_job),
-                           (size_t)(1 + p.tile_ctas) * 4};
-  size_t at[12] = {0};
-  for (int i = 0; i < 11; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
-  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[11]);
+                           (size_t)(1 + p.tile_ctas) * 4, out_dtype == QENG_F32 ? (size_t)p.tile_ctas * 256 * kHD * 4 : 0};
+  size_t at[13] = {0};
+  for (int i = 0; i < 12; ++i) at[i + 1] = at[i] + ((need[i] + 255) & ~(size_t)255);
+  rc = qeng_scratch_grow(ctx, sc, &sc->shared, at[12]);
   if (rc != QENG_OK) return rc;
   unsigned char* const mem = static_cast<unsigned char*>(sc->shared.ptr);
   p.tile_first = reinterpret_cast<int*>(mem);
@@ -1311,6 +1363,7 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   p.tile_jobs = reinterpret_cast<qeng_tile_job*>(mem + at[8]);
   p.own_jobs = reinterpret_cast<qeng_own_job*>(mem + at[9]);
   p.tile_list = reinterpret_cast<int*>(mem + at[10]);
+  p.kept_o = reinterpret_cast<float*>(mem + at[11]);
   if (out_dtype == QENG_F32) attn_tile_kernel<true><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   else attn_tile_kernel<false><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   QENG_LAUNCH_CHECK(ctx);

@@ -40,6 +40,7 @@ struct qeng_shared_attn {
   long long* unit_first;       // [T + 1] units (of one kv head) of the rows before a row: own pages, and what a start costs
   qeng_tile_job* tile_jobs;    // [tile_ctas]
   qeng_own_job* own_jobs;      // [own_warps]
+  float* kept_o;               // f32 results: [tile_ctas][32 x 4 dims][256], what a CTA has added up of its double tile
   int* tile_list;              // how many tile jobs there are, and whose
   float *cut_o, *cut_ml;       // cut between warps: [2 own_warps][8][128], [..][2]
 };

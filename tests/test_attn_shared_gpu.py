@@ -504,3 +504,75 @@ def test_from_request_lengths_to_attention(ctx):
     for _ in range(3):
         step([1, 1, 40, 1, 1], ([0, 2, 42, 44], [6, 6, 6]))
     pool.free()
+
+
+def test_long_sums_of_f32_results(ctx):
+    """Many blocks to a CTA: the MMAs cut the sums they add to, 2^-23 of them at most, and a sum is added to 32 times before it is rounded
+    to nearest in memory (without that the error grows with the blocks, beyond 10^-5 here); 2^-21 for scores and weights."""
+    import torch
+    b = Batch(ctx, [(3000, [48000 - i for i in range(40)])], 32, 8)
+    a, kw = b.args()
+    got = ctx.attn_shared(*a, **kw)
+    want, _ = b.exact()
+    assert float((got.double() - want).norm() / want.norm()) < 32 * 2.0 ** -23 + 2.0 ** -21
+    b.pool.free()
+
+
+def test_many_rows(ctx):
+    """30000 rows in 700 groups, some without pages, some without company, against the decode attention of every row by itself."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rows, pages, width, hkv = 30000, 4000, 9, 2
+    pool = ctx.kv_pool(pages, hkv)
+    data = pool.tensor()
+    data.copy_(torch.randn(data.shape, generator=g, device="cuda").half())
+    table = torch.randint(0, pages, (rows, width), generator=g, device="cuda", dtype=torch.int32)
+    first = torch.cat([torch.tensor([0], device="cuda"), torch.randint(0, rows + 1, (699,), generator=g, device="cuda").sort().values, torch.tensor([rows], device="cuda")])
+    shared = torch.randint(-3, width + 1, (700,), generator=g, device="cuda").clamp(min=0)
+    of = torch.searchsorted(first[1:], torch.arange(rows, device="cuda"), right=True)
+    head = table[first[:-1].clamp(max=rows - 1)][of]  # every row begins with its group's first pages
+    table = torch.where(torch.arange(width, device="cuda") < shared[of][:, None], head, table).contiguous()
+    lens = torch.randint(0, width * PAGE + 1, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    lens[::7] = 0
+    q = torch.randn(rows, 4, HD, generator=g, device="cuda").half()
+    i32 = torch.int32
+    for window in (0, 30):
+        got = ctx.attn_shared(pool, q, table, lens, first.to(i32), shared.to(i32), window=window)
+        want = ctx.attn_decode(pool, q, table, lens, window=window)
+        assert float((got - want).abs().max()) < 1e-4 * float(want.abs().max())
+    ctx.device_status()
+    pool.free()
+
+
+def test_contexts_of_two_threads(ctx):
+    """Two contexts on one device, each with its stream and thread, over one pool."""
+    import threading
+    import torch
+    from cyb_b200 import qeng
+    b = Batch(ctx, [behind(50, [7 * i for i in range(40)]), (12, list(range(1, 193)))], 16, 4)
+    a, kw = b.args()
+    want, mag = b.exact()
+    torch.cuda.synchronize()
+    outs, bad = [[], []], []
+
+    def work(k):
+        try:
+            c = qeng.Context(0)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(15):
+                    outs[k].append(c.attn_shared(*a, **kw))
+                torch.cuda.current_stream().synchronize()
+            c.device_status()
+            c.close()
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+    for got in outs[0] + outs[1]:
+        assert torch.equal(got, outs[0][0])
+    assert_near(outs[0][0], want, mag)
+    b.pool.free()
