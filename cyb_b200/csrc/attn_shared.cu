@@ -243,12 +243,21 @@ __device__ __forceinline__ void add_pieces(int lane, int c0, int c1, const float
 
 // ---- shared pages -------------------------------------------------------------------------------------------------------------
 // A double tile is two tiles of 128 MMA rows, each of `tokens` tokens x the query heads of a kv head, against the same keys, 128 (eight
-// pages) at a time.  Queries, K and V lie in shared memory, the scores S (two times 64 keys) and the outputs O in tensor memory (256 columns a
-// tile); the weights P take the place of the scores, as one f16 number or two (f32 results).  Warps 0-3 and 4-7 are the softmax of the two tiles, a
-// lane a row; 8 issues the MMAs, 9 the copies, 10 and 11 look for values that are not finite.  The MMAs of 64 keys run beside
-// the softmax of the next and of the other tile.  O is rescaled only when a row's maximum has grown by more than 2^kGrow since it was last.
+// pages) at a time.  Queries, K and V lie in shared memory, the scores S and the outputs O in tensor memory (256 columns
+// a tile); the weights P take the place of the scores, as one f16 number or two (f32 results).  Warps 0-3 and 4-7 are the softmax of the
+// two tiles, a lane a row; 8 issues the MMAs, 9 the copies, 10 and 11 look for values that are not finite.  The weights are handed over
+// 64 keys at a time, the second ones first; the MMAs of one tile run beside the softmax of the other.  O is rescaled only when a row's
+// maximum has grown by more than 2^kGrow since it was last.
 //
 // K and V tiles: [2 halves of 64 dims][128 keys][128 bytes], 128-byte swizzled; K is a K-major operand of 128 columns, V an MN-major one.
+//
+// Bound by the chain of a tile: 128 keys of both tiles take 3550 cycles, of which the MMAs need 2048 and the powers of two as many (16 a
+// cycle and SM); a tile's softmax takes 2150 of them and then waits 1400 for its values and the next scores.  256 rows behind 16384 tokens,
+// 32 query and 8 kv heads: 78 us (69 GFLOP, 0.53 of the measured rate; the tensor pipe is busy for 44 % of the cycles).  What did not
+// help, each measured against the kernel of its time: eight softmax warps a tile (96 registers and spills: 110 us, 92 without), a warp of
+// its own for each tile's MMAs (the tiles fall into step and wait together: 4900 cycles for 128 keys), scores of 64 keys in two buffers
+// (an MMA of 64 columns takes 74 cycles: 107 us, 92 without), part of the powers as polynomials on the FMA pipe (a call 133 us, 129
+// without).
 constexpr int kRows = 128, kKeys = 128;
 constexpr uint32_t kTileBytes = kRows * kHD * 2, kHalf = kTileBytes / 2;
 constexpr int kSoftWarps = 8, kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + 1, kCheckWarp = kLoadWarp + 1, kCheckWarps = 2;
@@ -915,8 +924,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 }
 
 // ---- a row's own pages ------------------------------------------------------------------------------------------------------
-// Every warp has pages of its own, of one or several (row, kv head), and keeps two on their way.  The query heads of the kv head are
-// the eight columns of every MMA, S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
+// Every warp has pages of its own, of one or several (row, kv head), and keeps two on their way.  HBM-bound where there are many pages:
+// 256 rows of 1 to 256 tokens (134 MB) take 29 us (4.6 TB/s), 64 of 1 to 1024 27 us; below that a start and an end, 4 to 5 us, and 1 us
+// a page.  With a (row, kv head) for the four warps of a CTA, merged in shared memory, these took 57 and 48 us.  The query heads of the
+// kv head are the eight columns of every MMA, S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
 __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   extern __shared__ unsigned char smem_raw[];
@@ -1174,6 +1185,8 @@ __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared
 
 // ---- what was cut: a CTA of attn_tile_kernel left a job for the double tile (and kv head) that it ends with, a warp of
 // attn_own_kernel for its last (row, kv head).  A tile's job also takes its rows' own sums, cut or whole.
+// Bound by the latency of its loads: 5 to 13 us.  80 registers hold four pieces on their way; 64 for one more CTA took a call of 64 rows
+// behind 16384 tokens from 80 to 85 us, 128 for eight pieces one of seven prompts from 395 to 409.
 constexpr int kJoinWarps = 8, kJoinParts = 16;  // CTAs to a tile's job: a warp has eight of its 256 rows and a quarter of their dims
 
 __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const qeng_shared_attn p) {

@@ -4,10 +4,12 @@
 // kv_plan_kernel: everything follows from three exclusive sums over the requests (tokens, pages taken, pages given back), which
 // every CTA computes for itself in shared memory; a token or page finds its request by bisection there.  One CTA, or a cluster of up
 // to eight where the buffers are long: lengths and counters may be updated in place, so nobody writes them before every CTA has read
-// them, and a cluster's barrier is the cheapest place to wait for that.
+// them, and a cluster's barrier is the cheapest place to wait for that.  Bound by latency: 64 requests 5.6 us, 1000 with 131072 places
+// for tokens 13.6 us (2 MB written; 26 us before a page id was asked for once for four tokens, stores had 16 bytes and blocks grew with the call).
 //
 // rope_append_slots_kernel: HBM-bound, (Hq + 2 Hkv) * 128 values read and written as f16 once.  A CTA has a token; sixteen lanes have
-// a head (the pairs (i, i + 64) of a lane are eight values: 16-byte loads of f32 rows).
+// a head (the pairs (i, i + 64) of a lane are eight values: 16-byte loads of f32 rows).  8192 rows of 48 f32 heads:
+// 49.5 us, 6.1 TB/s (57 with the slot asked for before the row).
 #include <math.h>
 
 #include "qeng_internal.h"

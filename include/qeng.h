@@ -88,7 +88,8 @@ int32_t qeng_destroy(qeng_ctx* ctx);
 const char* qeng_last_error(const qeng_ctx* ctx);
 /* Drain the device, read and clear the status word kernels write when they meet a
  * malformed input (page id outside the pool, position outside the cache, token
- * outside the vocabulary): QENG_OK or QENG_ERR_DEVICE_STATUS. */
+ * outside the vocabulary, counters of a page ring or bounds of row groups that make no
+ * sense): QENG_OK or QENG_ERR_DEVICE_STATUS. */
 int32_t qeng_device_status(qeng_ctx* ctx);
 /* SM count of the context's device (grid sizing, reporting). */
 int32_t qeng_sm_count(const qeng_ctx* ctx);
@@ -306,8 +307,9 @@ int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int
  *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.
  *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
  *    results of the rows that attend it infinite or NaN, and of no other row.
- * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do not ascend, and rows outside the table, are
- * reported (status 6; with such bounds nothing is written).  Needs working memory of the context. */
+ * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do
+ * not ascend, and rows outside the table, are reported (status 6; with such bounds nothing is written).  Needs working memory of the
+ * context: 520 * T * Hq bytes and, on 148 SMs, 54 MB (73 for f32 results). */
 int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, const uint16_t* q_f16, int64_t ldq,
                          const int32_t* page_table, int64_t max_pages, int64_t table_rows, const int32_t* rows,
                          const int32_t* lens, int64_t T, int64_t Hq, const int32_t* group_first,
