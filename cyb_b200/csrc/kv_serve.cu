@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) rope_append_slots_kernel(co
   __syncthreads();
   const float4 c = *reinterpret_cast<const float4*>(&cs[0][4 * l]), s = *reinterpret_cast<const float4*>(&cs[1][4 * l]);
   __half* const page = p.pool + (size_t)(slot / kPage) * p.Hkv * (2 * kPage * kHD) + slot % kPage * kHD + 4 * l;
-  for (int h0 = lane_head; h0 < heads; h0 += kAtOnce * kStep) {
+  // both halves of a warp go round together, though with an odd number of heads the second has none at the end
+  for (int h0 = lane_head; h0 - lane_head % 2 < heads; h0 += kAtOnce * kStep) {
     if (h0 != lane_head) load(h0);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
