@@ -414,6 +414,9 @@ class Context:
         assert add.numel() == n and rows >= n and (keep is None or keep.numel() == n)
         if out is None:
             out = self.kv_plan_buffers(n, capacity)
+        for t in out[:6]:
+            assert t.is_cuda and t.dtype is i32 and t.is_contiguous()
+        assert out.ends.is_cuda and out.ends.dtype is torch.int64 and out.ends.is_contiguous() and out.ends.numel() == 2
         assert out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
         rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), width,
                                ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
@@ -431,11 +434,11 @@ class Context:
         hq = width // hd - 2 * pool.kv_heads
         ld, one = qkv.stride()
         assert qkv.is_cuda and one == 1 and width % hd == 0
-        assert pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
+        assert pos.is_cuda and slots.is_cuda and pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
         if out is None:
             out = qkv.new_empty((t, hq, hd), dtype=torch.float16)
         ldq, per_head, per_dim = out.stride()
-        assert out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
+        assert out.is_cuda and out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
         rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), _dtype(qkv), t, ld if t > 1 else width, hq,
                                    None if q_gain is None else _gain(q_gain), None if k_gain is None else _gain(k_gain), eps, pos.data_ptr(),
                                    slots.data_ptr(), base, out.data_ptr(), ldq if t > 1 else hq * hd, _cur_stream())
@@ -451,7 +454,7 @@ class Context:
         import torch
         (t, hq, hd), i32 = q.shape, torch.int32
         ldq, per_head, per_dim = q.stride()
-        assert q.dtype is torch.float16 and per_dim == 1 and per_head == hd
+        assert q.is_cuda and q.dtype is torch.float16 and per_dim == 1 and per_head == hd
         for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
             assert x.is_cuda and x.dtype is i32 and x.is_contiguous()
         (table_rows, width), g = table.shape, group_pages.numel()
@@ -459,7 +462,7 @@ class Context:
         if out is None:
             out = q.new_empty((t, hq, hd), dtype=dtype or torch.float32)
         ldo, per_head, per_dim = out.stride()
-        assert out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
+        assert out.is_cuda and out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
         rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), ldq if t > 1 else hq * hd, table.data_ptr(), width, table_rows,
                                    None if rows is None else rows.data_ptr(), lens.data_ptr(), t, hq, group_first.data_ptr(), group_pages.data_ptr(), g,
                                    float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(), _dtype(out), ldo if t > 1 else hq * hd,
