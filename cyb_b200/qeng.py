@@ -414,10 +414,8 @@ class Context:
         assert add.numel() == n and rows >= n and (keep is None or keep.numel() == n)
         if out is None:
             out = self.kv_plan_buffers(n, capacity)
-        for t in out[:6]:
-            assert t.is_cuda and t.dtype is i32 and t.is_contiguous()
-        assert out.ends.is_cuda and out.ends.dtype is torch.int64 and out.ends.is_contiguous() and out.ends.numel() == 2
-        assert out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
+        assert isinstance(out, KVPlan)  # its tensors were looked at when it was made
+        assert out.ends.numel() == 2 and out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
         rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), width,
                                ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
                                out.slots.data_ptr(), out.pos.data_ptr(), out.seen.data_ptr(), out.rows.data_ptr(), capacity, _cur_stream())
@@ -492,9 +490,7 @@ def _gain(t):
     return t.data_ptr()
 
 
-class KVPlan(NamedTuple):
-    """What kv_plan works out: tokens of a request are starts[r] .. starts[r + 1] - 1; per token its slot, position, number of keys
-    attended and request; lengths and ring counters afterwards."""
+class _PlanFields(NamedTuple):
     starts: object
     slots: object
     pos: object
@@ -502,6 +498,26 @@ class KVPlan(NamedTuple):
     rows: object
     lens: object
     ends: object
+
+
+class KVPlan(_PlanFields):
+    """What kv_plan works out: tokens of a request are starts[r] .. starts[r + 1] - 1; per token its slot, position, number of keys
+    attended and request; lengths and ring counters afterwards.  Contiguous tensors of the device, int32 but for the counters (int64);
+    _replace(lens=..., ends=...) makes a plan that updates a caller's tensors in place."""
+    __slots__ = ()
+
+    def __new__(cls, *args, **kw):
+        return super().__new__(cls, *args, **kw)._checked()
+
+    @classmethod
+    def _make(cls, values):  # _replace comes through here
+        return super()._make(values)._checked()
+
+    def _checked(self):
+        import torch
+        for t in self:
+            assert t.is_cuda and t.is_contiguous() and t.dtype is (torch.int64 if t is self.ends else torch.int32)
+        return self
 
 
 class Weight:

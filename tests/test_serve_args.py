@@ -96,6 +96,17 @@ def test_a_tensor_of_another_type_is_refused(lib, ctx, call, args, name):
     assert not lib.calls
 
 
+def test_a_plan_with_a_tensor_replaced_is_looked_at_again(lib, ctx):
+    a = plan_args()
+    out = qeng.KVPlan(a["starts"], a["slots"], a["pos"], a["seen"], a["rows"], a["lens_out"], a["ends_out"])
+    assert out._replace(lens=a["lens"]).lens is a["lens"]
+    with pytest.raises(AssertionError):
+        out._replace(lens=a["lens"].as_subclass(torch.Tensor))
+    with pytest.raises(AssertionError):
+        ctx.kv_plan(Pool, a["lens"], a["add"], a["table"], a["ring"], a["ends"], 8, out=tuple(out))
+    assert not lib.calls
+
+
 @pytest.mark.parametrize("name", ["starts", "slots", "pos", "seen", "rows", "lens_out", "ends_out"])
 def test_a_broadcast_result_of_the_plan_is_refused(lib, ctx, name):
     a = plan_args()
