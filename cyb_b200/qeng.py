@@ -565,6 +565,16 @@ class Weight:
             pass
 
 
+class _PoolMemory:
+    """What torch makes a view of a pool from, and what the view then holds: an object without cycles, so that the pool's memory goes
+    with the last view and not when a collector comes round."""
+
+    def __init__(self, pool):
+        n = pool.pages * pool.kv_heads * 2 * 16 * pool.hd
+        self.pool = pool
+        self.__cuda_array_interface__ = {"shape": (n,), "typestr": "<f2", "data": (_lib.qeng_kv_pool_data(pool.h), False), "version": 2}
+
+
 class KVPool:
     def __init__(self, ctx, h, pages, kv_heads, hd):
         self.ctx, self.h, self.pages, self.kv_heads, self.hd = ctx, h, pages, kv_heads, hd
@@ -573,14 +583,7 @@ class KVPool:
         """The pool's storage as a torch f16 view [pages, kv_heads, 2, 16, hd].  The pool stays while a view of it does, unless it is
         freed by hand."""
         import torch
-        n = self.pages * self.kv_heads * 2 * 16 * self.hd
-        ptr = _lib.qeng_kv_pool_data(self.h)
-        iface = {"shape": (n,), "typestr": "<f2", "data": (ptr, False), "version": 2}
-
-        class _Holder:
-            __cuda_array_interface__ = iface
-            pool = self
-        return torch.as_tensor(_Holder(), device="cuda:%d" % self.ctx.device).view(self.pages, self.kv_heads, 2, 16, self.hd)
+        return torch.as_tensor(_PoolMemory(self), device="cuda:%d" % self.ctx.device).view(self.pages, self.kv_heads, 2, 16, self.hd)
 
     def free(self):
         if self.h:
