@@ -22,14 +22,6 @@ static const size_t kStatusBytes = 256 + 8 * (8 + 30000 * 8);
 static const size_t kStatusBytes = 256;
 #endif
 
-// Allocations are no part of any graph: they are made outside the thread's capture mode, so that a call inside a capture,
-// or beside one on another stream, may make its working memory.
-struct OutsideCapture {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
-
 static void free_scratch(qeng_scratch* sc) {
   OutsideCapture outside;
   for (void* p : sc->kept) cudaFree(p);

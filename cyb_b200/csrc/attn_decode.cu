@@ -585,6 +585,7 @@ int32_t qeng_kv_pool_create(qeng_ctx* ctx, int64_t pages, int64_t kv_heads, int6
 int32_t qeng_kv_pool_free(qeng_ctx* ctx, qeng_kv_pool* pool) {
   if (!pool) return QENG_OK;
   if (ctx) cudaSetDevice(ctx->device);
+  OutsideCapture outside;  // a host's collector may free it at any time
   if (pool->data) cudaFree(pool->data);
   delete pool;
   return QENG_OK;

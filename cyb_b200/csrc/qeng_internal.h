@@ -104,6 +104,14 @@ struct qeng_ctx {
   int32_t* tail_cnt = nullptr;
 };
 
+// Allocations are no part of any graph: they are made outside the thread's capture mode, so that a call inside a capture,
+// or beside one on another stream, may make its working memory, and a pool may be freed meanwhile.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 int32_t qeng_fail(qeng_ctx* ctx, int32_t code, const char* fmt, ...);
 
 #define QENG_CUDA(ctx, expr)                                                              \

@@ -69,3 +69,26 @@ def test_a_view_of_the_device_keeps_its_pool_no_longer_than_it_lives(ctx, collec
     assert alive() is not None and bool((view == 2).all())
     del view
     assert alive() is None
+
+
+@pytest.mark.gpu
+def test_a_pool_may_be_freed_while_a_stream_is_captured(ctx):
+    """As a collector may do at any allocation: the capture stays valid, and the memory is given back."""
+    before = torch.cuda.mem_get_info()[0]
+    pool, kept = ctx.kv_pool(4096, 8), ctx.kv_pool(2, 1)
+    assert torch.cuda.mem_get_info()[0] <= before - 4096 * 8 * 8192
+    x = torch.arange(3 * 128, device="cuda", dtype=torch.float32).view(1, 384) / 128
+    pos, slots, q = (torch.zeros(1, dtype=t, device="cuda") for t in (torch.int32, torch.int32, torch.float16))
+    q = q.expand(128).contiguous().view(1, 1, 128)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ctx.rope_append(kept, x, pos, slots, 1e4, out=q)
+        del pool
+        ctx.rope_append(kept, x, pos, slots, 1e4, out=q)
+    assert torch.cuda.mem_get_info()[0] > before - 4096 * 8 * 8192
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(q.view(-1), x[0, :128].half())
+    kept.free()
+    ctx.device_status()
