@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         // their weights, where the compiler would otherwise put those in front.
         float s[64];
         const auto scores = [&](int half) {
+          __syncwarp();  // one lane has let the MMAs go on with the other half
           tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
           if (p.softcap > 0.f) {
 #pragma unroll
@@ -744,6 +745,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           l_run *= alpha;
           scale_kept *= alpha;
           if (j > 0) {  // the values of the block before are in (its scores came behind them), the next wait for this warp
+            __syncwarp();  // not every lane's reference has moved
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
@@ -756,6 +758,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
         }
         if (kTwo && fresh && j > 0) {
           st_wait();
+          __syncwarp();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float4 before[8];
