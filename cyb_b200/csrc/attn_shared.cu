@@ -503,13 +503,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
       int id = lane < 16 && w.page0 + pg <= last_page ? ids[w.page0 + pg] : 0;
       for (int j = 0; j < w.blocks && !failed; ++j, ++b) {
         const int here = w.page0 + j * 8, pages = min(8, last_page - here + 1);
-        int row = id;
-        if ((unsigned)row >= (unsigned)p.pool_pages) {  // malformed page table: record it, read a page that exists
-          atomicExch(p.status, 1);
-          row = 0;
-        }
+        int row = -64;  // in front of the pool: the copies bring zeros
+        if ((unsigned)id < (unsigned)p.pool_pages) row = (id * p.Hkv + w.h) * 32;
+        else atomicExch(p.status, 1);  // malformed page table
         if (lane < 16 && j + 1 < w.blocks && here + 8 + pg <= last_page) id = ids[here + 8 + pg];
-        row = (row * p.Hkv + w.h) * 32;
         for (int kv = 0; kv < 2; ++kv) {
           const int slot = 2 * (b & 1) + kv;
           const uint32_t bar = smem_u32(sh.full + slot);
@@ -840,8 +837,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
               }
               const bool on = key >= begin && key < end;
               const int id = p.table[(size_t)w.table_row * p.max_pages + key / kPage];
-              const __half2* const val = reinterpret_cast<const __half2*>(
-                  p.pool + (((size_t)((unsigned)id < (unsigned)p.pool_pages ? id : 0) * p.Hkv + w.h) * 32 + 16 + key % kPage) * kHD);
+              if ((unsigned)id >= (unsigned)p.pool_pages) continue;  // (its place holds zeros, and is not looked up)
+              const __half2* const val = reinterpret_cast<const __half2*>(p.pool + (((size_t)id * p.Hkv + w.h) * 32 + 16 + key % kPage) * kHD);
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];

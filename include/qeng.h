@@ -308,7 +308,8 @@ int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int
  *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
  *    results of the rows that attend it infinite or NaN, and of no other row.
  * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do
- * not ascend, and rows outside the table, are reported (status 6; with such bounds nothing is written).  Needs working memory of the
+ * not ascend, and rows outside the table, are reported (status 6; with such bounds nothing is written).  A page id outside the pool is
+ * reported (status 1): no page is read in its place, and what the rows that attend it get means nothing.  Needs working memory of the
  * context: 520 * T * Hq bytes and, on 148 SMs, 54 MB (73 for f32 results). */
 int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, const uint16_t* q_f16, int64_t ldq,
                          const int32_t* page_table, int64_t max_pages, int64_t table_rows, const int32_t* rows,
