@@ -215,7 +215,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanParams 
   for (int i = self; i < given; i += all) {
     const int r = find_row(back, 0, p.R, i);
     // the request's pages end with its last one
-    p.ring[ring_at(t0, i)] = p.table[(size_t)r * p.max_pages + (len[r] + kPage - 1) / kPage - (back[r + 1] - i)];
+    const int id = p.table[(size_t)r * p.max_pages + (len[r] + kPage - 1) / kPage - (back[r + 1] - i)];
+    if ((unsigned)id >= (unsigned)p.pages) atomicExch(p.status, 1);  // the counters go on, and so it stands in the ring
+    p.ring[ring_at(t0, i)] = id;
   }
   for (int r = self; r <= p.R; r += all) p.starts[r] = tok[r];
   if (p.ctas > 1) cluster_wait();  // everybody has: they may be overwritten

@@ -283,8 +283,9 @@ int32_t qeng_attn_decode_noalloc(qeng_ctx* ctx, const qeng_kv_pool* pool, const 
  *  - starts[R + 1]: the first token of every request, and their number; per token up to `capacity`: slots (16 * page + place in the
  *    page), pos (its position), seen (pos + 1: the keys it attends), rows (its request).  Entries behind the last token are -1, 0, 0, -1.
  *  - lens_out, ends_out: lengths and counters afterwards.  They may be lens and ends themselves.
- * A page id outside the pool is reported (status 1), the slots in it are -1; so are counters that make no sense, or more pages given
- * back than the ring has room for (status 6; then nothing is given back).  At most 8192 requests. */
+ * A page id outside the pool is reported (status 1): the slots in such a page are -1, and one that is given back goes into the ring as it
+ * stands.  Counters that make no sense, or more pages given back than the ring has room for, are reported, too (status 6; then nothing is
+ * given back).  At most 8192 requests. */
 int32_t qeng_kv_plan(qeng_ctx* ctx, const qeng_kv_pool* pool, int64_t R, const int32_t* lens, const int32_t* add,
                      const int32_t* keep, int32_t* page_table, int64_t max_pages, int32_t* ring, int64_t ring_size,
                      const int64_t* ends, int32_t* lens_out, int64_t* ends_out, int32_t* starts, int32_t* slots,
