@@ -53,10 +53,13 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
-// cap * tanh(y), cap2 x = 2 y log2(e): 1 - 2 / (e^2y + 1), its error 2^-22 of the cap
+// cap * tanh(y), cap2 x = 2 y log2(e): 1 - 2 / (e^2y + 1), its error 2^-22 of the cap, however small the score.  Weights of 11 bits
+// are off by 2^-12 themselves: results of 16 bits take this form for caps up to kCoarseCap, where a score, and so a weight, is off by 2^-14.
+constexpr float kCoarseCap = 256.f;
 __device__ __forceinline__ float capped(float x, float cap2, float cap) { return fmaf(-2.f * cap, rcp(ex2(x * cap2) + 1.f), cap); }
-// The same for f32 results: below 0.6, where scores mostly are and the difference above cancels, y + y^3 P(y^2), P fitted at Chebyshev
-// nodes (relative error 2^-23.6).
+// The same for f32 results and larger caps: below 0.6, where scores mostly are and the difference above cancels, y + y^3 P(y^2), P fitted at Chebyshev
+// nodes (relative error 2^-23.6).  With it for all caps, calls of 16-bit results at a cap of 50 took 42 us for 37, 295 for 222 (256 rows
+// behind 16384 tokens) and 1007 for 694 (seven prompts); with both forms in one kernel 38, 228 and 699.
 __device__ __forceinline__ float capped_f32(float x, float cap2, float cap) {
   const float y = x * (cap2 * 0.34657359027997264f), z = y * y;  // ln(2) / 2
   float p = fmaf(-0.006276387721f, z, 0.02111621387f);
@@ -355,7 +358,7 @@ struct TileShared {
   uint64_t pfull[2], pempty[2], qfull, qempty, full[4], empty[4], sdone[2], odone[2], pready[2][2], checked[2], drained;
 };
 
-template <bool kTwo>  // weights as two f16 numbers
+template <bool kTwo, bool kFineCap>  // weights as two f16 numbers; scores capped by capped_f32
 __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap, const __grid_constant__ CUtensorMap qmap) {
   extern __shared__ unsigned char smem_raw[];
   const uint32_t qs = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = qs + 2 * kTileBytes;
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
           tmem_ld64(mem + 64 * half, reinterpret_cast<uint32_t*>(s));
           if (p.softcap > 0.f) {
 #pragma unroll
-            for (int k = 0; k < 64; ++k) s[k] = kTwo ? capped_f32(s[k], cap2, cap) : capped(s[k], cap2, cap);
+            for (int k = 0; k < 64; ++k) s[k] = kFineCap ? capped_f32(s[k], cap2, cap) : capped(s[k], cap2, cap);
           }
           if (edge) {
             const int e = end - key0 - 64 * half, a = begin - key0 - 64 * half;
@@ -1336,8 +1339,8 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   static bool configured_on[64] = {};  // the opt-in shared-memory size is set per device
   bool& configured = configured_on[ctx->device & 63];
   if (!configured) {
-    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_tile_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTileSmem + groups_bytes(kSharedGroups))));
-    QENG_CUDA(ctx, cudaFuncSetAttribute(attn_tile_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTileSmem + groups_bytes(kSharedGroups))));
+    for (auto* const fn : {attn_tile_kernel<false, false>, attn_tile_kernel<false, true>, attn_tile_kernel<true, true>})
+      QENG_CUDA(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTileSmem + groups_bytes(kSharedGroups))));
     QENG_CUDA(ctx, cudaFuncSetAttribute(attn_own_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kOwnSmem + groups_bytes(kSharedGroups))));
     configured = true;
   }
@@ -1377,8 +1380,8 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   p.own_jobs = reinterpret_cast<qeng_own_job*>(mem + at[9]);
   p.tile_list = reinterpret_cast<int*>(mem + at[10]);
   p.kept_o = reinterpret_cast<float*>(mem + at[11]);
-  if (out_dtype == QENG_F32) attn_tile_kernel<true><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
-  else attn_tile_kernel<false><<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
+  auto* const tile_kernel = out_dtype == QENG_F32 ? attn_tile_kernel<true, true> : softcap > kCoarseCap ? attn_tile_kernel<false, true> : attn_tile_kernel<false, false>;
+  tile_kernel<<<(unsigned)p.tile_ctas, kTileThreads, kTileSmem + groups_bytes(G), st>>>(p, tile_map, q_map);
   QENG_LAUNCH_CHECK(ctx);
   // the other two may start as CTAs of the one in front leave
   cudaLaunchAttribute attr[1];

@@ -1,9 +1,9 @@
-"""Attention of rows that share pages: page ids outside the pool."""
+"""Attention of rows that share pages: caps of any size, page ids outside the pool."""
 import math
 
 import pytest
 
-from test_attn_shared_gpu import PAGE, Batch, _ints, assert_near, behind
+from test_attn_shared_gpu import PAGE, Batch, _ints, assert_near, behind, check
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,11 @@ def test_a_page_outside_the_pool_is_nobodys_page(ctx, bad, dtype):
         sound = [t for t, n in enumerate(b.lens) if n <= at * PAGE or (window and n - window >= (at + 1) * PAGE) or (not shared and t != 0)]
         assert_near(got[0][sound], want[sound], mag[sound])
         b.pool.free()
+
+
+@pytest.mark.parametrize("softcap", [0.25, 200.0, 256.0, 257.0, 1e3, 1e5, 1e8, 1e20])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_caps_far_from_the_scores(ctx, dtype, softcap):
+    """A cap bends scores near it and leaves those far below alone: no error that grows with the cap."""
+    check(ctx, [behind(21, [0, 1, 90, 33]), behind(0, [40]), behind(9, [3] * 70)], 12, 4, dtype, softcap=softcap)
+    check(ctx, [(30, list(range(1, 470)))], 8, 2, dtype, softcap=softcap, prompts=True, window=333)
