@@ -1321,6 +1321,8 @@ extern "C" int32_t qeng_attn_shared(qeng_ctx* ctx, const qeng_kv_pool* pool, con
   if (!ctx || !pool || !q_f16 || !page_table || !lens || !group_first || !group_pages || !out) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: null argument");
   if (T <= 0 || Hq <= 0 || max_pages <= 0 || table_rows <= 0 || G <= 0) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: T, Hq, G and the table's sizes must be positive");
   if (!(scale >= 0.f) || !(softcap >= 0.f) || window < 0) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: scale, softcap and window must not be negative");
+  if (softcap > 1e30f || (softcap > 0.f && !isfinite(2.f * kLog2e * scale / softcap)))
+    return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: softcap of %g with a scale of %g leaves 32 bits", softcap, scale);
   if (out_dtype < QENG_F32 || out_dtype > QENG_BF16) return qeng_fail(ctx, QENG_ERR_ARG, "attn_shared: unknown type %d", out_dtype);
   if (Hq % pool->kv_heads != 0 || Hq / pool->kv_heads > 8)
     return qeng_fail(ctx, QENG_ERR_SHAPE, "attn_shared: query heads per kv head must divide evenly and be <= 8");

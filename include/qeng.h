@@ -305,7 +305,8 @@ int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int
  * request, lens[t] = position + 1: what qeng_kv_plan writes), and a row without company is a group of one with no page shared.
  *  - q_f16[t] and out[t] (f32, f16 or bf16) are [Hq][128], ldq and ldo values from row to row.  rows may be NULL: row t has table
  *    row t.  A row in no group, or with rows[t] < 0, is left alone; one that attends nothing (lens[t] <= 0) gives zeros.
- *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.
+ *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.  softcap is at most 1e30, and scale / softcap
+ *    10^38 (QENG_ERR_ARG).
  *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
  *    results of the rows that attend it infinite or NaN, and of no other row.
  * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do

@@ -57,3 +57,16 @@ def test_caps_far_from_the_scores(ctx, dtype, softcap):
     """A cap bends scores near it and leaves those far below alone: no error that grows with the cap."""
     check(ctx, [behind(21, [0, 1, 90, 33]), behind(0, [40]), behind(9, [3] * 70)], 12, 4, dtype, softcap=softcap)
     check(ctx, [(30, list(range(1, 470)))], 8, 2, dtype, softcap=softcap, prompts=True, window=333)
+
+
+def test_caps_that_leave_32_bits_are_refused(ctx):
+    """An infinite one, or one far below what scores are: rows would be NaN."""
+    from cyb_b200 import qeng
+    b = Batch(ctx, [behind(3, [5])], 8, 2)
+    a, kw = b.args()
+    for cap, scale in ((math.inf, 1.0), (2e30, 1.0), (1e-39, 1.0), (1e-30, 1e9)):
+        with pytest.raises(qeng.QengError, match="leaves 32 bits"):
+            ctx.attn_shared(*a, **kw, softcap=cap, scale=scale)
+    b.pool.free()
+    check(ctx, [behind(3, [5])], 8, 2, softcap=1e30)
+    check(ctx, [behind(3, [5])], 8, 2, softcap=1e-30, scale=1.0)
