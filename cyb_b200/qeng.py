@@ -452,7 +452,7 @@ class Context:
         import torch
         (t, hq, hd), i32 = q.shape, torch.int32
         ldq, per_head, per_dim = q.stride()
-        assert q.is_cuda and q.dtype is torch.float16 and per_dim == 1 and per_head == hd
+        assert q.is_cuda and q.dtype is torch.float16 and per_dim == 1 and per_head == hd == pool.hd
         for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
             assert x.is_cuda and x.dtype is i32 and x.is_contiguous()
         (table_rows, width), g = table.shape, group_pages.numel()
