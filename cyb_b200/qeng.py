@@ -394,6 +394,10 @@ class Context:
         return out
 
     # ---- serving -------------------------------------------------------------
+    @property
+    def _here(self):
+        return -1, self.device  # what get_device says of tensors that may be used; -1: of no GPU, as is_cuda tells
+
     def kv_plan_buffers(self, requests, capacity):
         """Buffers for the results of kv_plan, to be used again from step to step (and by a captured one)."""
         import torch
@@ -406,15 +410,15 @@ class Context:
         """Pages and slots for add[r] more tokens of every request, see qeng_kv_plan: the table and the ring are updated, the rest
         comes back as a KVPlan.  `out`: a KVPlan to fill; its lens and ends may be the arguments themselves."""
         import torch
-        i32, n = torch.int32, lens.numel()
+        i32, n, here = torch.int32, lens.numel(), self._here
         for t in (lens, add, table, ring) if keep is None else (lens, add, table, ring, keep):
-            assert t.is_cuda and t.dtype is i32 and t.is_contiguous()
-        assert ends.is_cuda and ends.dtype is torch.int64 and ends.is_contiguous() and ends.numel() == 2
+            assert t.is_cuda and t.get_device() in here and t.dtype is i32 and t.is_contiguous()
+        assert ends.is_cuda and ends.get_device() in here and ends.dtype is torch.int64 and ends.is_contiguous() and ends.numel() == 2
         rows, width = table.shape
         assert add.numel() == n and rows >= n and (keep is None or keep.numel() == n)
         if out is None:
             out = self.kv_plan_buffers(n, capacity)
-        assert isinstance(out, KVPlan)  # its tensors were looked at when it was made
+        assert isinstance(out, KVPlan) and out.ends.get_device() in here  # its tensors were looked at when it was made
         assert out.ends.numel() == 2 and out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
         rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), width,
                                ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
@@ -428,17 +432,17 @@ class Context:
         heads, rotation, k and v into the pool at `slots`; returns q as float16 [T, Hq, 128].  Rows with a negative slot are left alone
         (those of a new result are then not initialised)."""
         import torch
-        (t, width), hd, i32 = qkv.shape, pool.hd, torch.int32
+        (t, width), hd, i32, here = qkv.shape, pool.hd, torch.int32, self._here
         hq = width // hd - 2 * pool.kv_heads
         ld, one = qkv.stride()
-        assert qkv.is_cuda and one == 1 and width % hd == 0
-        assert pos.is_cuda and slots.is_cuda and pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
+        assert qkv.is_cuda and qkv.get_device() in here and one == 1 and width % hd == 0
+        assert pos.is_cuda and slots.is_cuda and pos.get_device() in here and slots.get_device() in here and pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
         if out is None:
             out = qkv.new_empty((t, hq, hd), dtype=torch.float16)
         ldq, per_head, per_dim = out.stride()
-        assert out.is_cuda and out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
+        assert out.is_cuda and out.get_device() in here and out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
         rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), _dtype(qkv), t, ld if t > 1 else width, hq,
-                                   None if q_gain is None else _gain(q_gain), None if k_gain is None else _gain(k_gain), eps, pos.data_ptr(),
+                                   None if q_gain is None else _gain(q_gain, here), None if k_gain is None else _gain(k_gain, here), eps, pos.data_ptr(),
                                    slots.data_ptr(), base, out.data_ptr(), ldq if t > 1 else hq * hd, _cur_stream())
         if rc:
             self.check(rc)
@@ -450,17 +454,17 @@ class Context:
         `dtype` (float32, float16 or bfloat16; None: float32); rows in no group, or of table row -1, are left alone (those of a new result
         are then not initialised)."""
         import torch
-        (t, hq, hd), i32 = q.shape, torch.int32
+        (t, hq, hd), i32, here = q.shape, torch.int32, self._here
         ldq, per_head, per_dim = q.stride()
-        assert q.is_cuda and q.dtype is torch.float16 and per_dim == 1 and per_head == hd == pool.hd
+        assert q.is_cuda and q.get_device() in here and q.dtype is torch.float16 and per_dim == 1 and per_head == hd == pool.hd
         for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
-            assert x.is_cuda and x.dtype is i32 and x.is_contiguous()
+            assert x.is_cuda and x.get_device() in here and x.dtype is i32 and x.is_contiguous()
         (table_rows, width), g = table.shape, group_pages.numel()
         assert lens.numel() == t and group_first.numel() == g + 1 and (rows is None or rows.numel() == t)
         if out is None:
             out = q.new_empty((t, hq, hd), dtype=dtype or torch.float32)
         ldo, per_head, per_dim = out.stride()
-        assert out.is_cuda and out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
+        assert out.is_cuda and out.get_device() in here and out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
         rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), ldq if t > 1 else hq * hd, table.data_ptr(), width, table_rows,
                                    None if rows is None else rows.data_ptr(), lens.data_ptr(), t, hq, group_first.data_ptr(), group_pages.data_ptr(), g,
                                    float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(), _dtype(out), ldo if t > 1 else hq * hd,
@@ -484,9 +488,9 @@ def _dtype(t):
     return _DTYPES[t.dtype]
 
 
-def _gain(t):
+def _gain(t, here):
     import torch
-    assert t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == 128
+    assert t.is_cuda and t.get_device() in here and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == 128
     return t.data_ptr()
 
 
@@ -502,7 +506,7 @@ class _PlanFields(NamedTuple):
 
 class KVPlan(_PlanFields):
     """What kv_plan works out: tokens of a request are starts[r] .. starts[r + 1] - 1; per token its slot, position, number of keys
-    attended and request; lengths and ring counters afterwards.  Contiguous tensors of the device, int32 but for the counters (int64);
+    attended and request; lengths and ring counters afterwards.  Contiguous tensors of one device, int32 but for the counters (int64);
     _replace(lens=..., ends=...) makes a plan that updates a caller's tensors in place."""
     __slots__ = ()
 
@@ -516,7 +520,7 @@ class KVPlan(_PlanFields):
     def _checked(self):
         import torch
         for t in self:
-            assert t.is_cuda and t.is_contiguous() and t.dtype is (torch.int64 if t is self.ends else torch.int32)
+            assert t.is_cuda and t.get_device() == self.ends.get_device() and t.is_contiguous() and t.dtype is (torch.int64 if t is self.ends else torch.int32)
         return self
 
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_serve_args import attn, attn_args, ctx, dev, lib  # noqa: F401
+from test_serve_args import CALLS, OnDevice, attn, attn_args, ctx, dev, lib  # noqa: F401
 
 
 @pytest.mark.parametrize("heads", [4, 32])
@@ -15,3 +15,28 @@ def test_heads_of_another_size_than_the_pools_are_refused(lib, ctx, heads, dims)
     with pytest.raises(AssertionError):
         attn(ctx, a)
     assert not lib.calls
+
+
+class Elsewhere(OnDevice):
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize("call,args,name", [(c, a, n) for c, a in CALLS for n in a()])
+def test_a_tensor_of_another_device_is_refused(lib, ctx, call, args, name):  # noqa: F811
+    a = args()
+    a[name] = a[name].as_subclass(Elsewhere)
+    with pytest.raises(AssertionError):
+        call(ctx, a)
+    assert not lib.calls
+
+
+@pytest.mark.parametrize("call,args", CALLS)
+def test_all_of_another_device_are_refused(lib, ctx, call, args):  # noqa: F811
+    a = {name: t.as_subclass(Elsewhere) for name, t in args().items()}
+    with pytest.raises(AssertionError):
+        call(ctx, a)
+    assert not lib.calls
+    ctx.device = 1
+    call(ctx, a)
+    assert len(lib.calls) == 1
