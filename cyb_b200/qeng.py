@@ -412,14 +412,19 @@ class Context:
         import torch
         i32, n, here = torch.int32, lens.numel(), self._here
         for t in (lens, add, table, ring) if keep is None else (lens, add, table, ring, keep):
-            assert t.is_cuda and t.get_device() in here and t.dtype is i32 and t.is_contiguous()
-        assert ends.is_cuda and ends.get_device() in here and ends.dtype is torch.int64 and ends.is_contiguous() and ends.numel() == 2
+            if not (t.is_cuda and t.get_device() in here and t.dtype is i32 and t.is_contiguous()):
+                raise AssertionError("kv_plan: lens, add, table, ring and keep are contiguous int32 tensors of the context's device")
+        if not (ends.is_cuda and ends.get_device() in here and ends.dtype is torch.int64 and ends.is_contiguous() and ends.numel() == 2):
+            raise AssertionError("kv_plan: ends is two contiguous int64 numbers on the context's device")
         rows, width = table.shape
-        assert add.numel() == n and rows >= n and (keep is None or keep.numel() == n)
+        if not (add.numel() == n and rows >= n and (keep is None or keep.numel() == n)):
+            raise AssertionError("kv_plan: lens, add, keep and the table's rows do not agree")
         if out is None:
             out = self.kv_plan_buffers(n, capacity)
-        assert isinstance(out, KVPlan) and out.ends.get_device() in here  # its tensors were looked at when it was made
-        assert out.ends.numel() == 2 and out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity
+        if not (isinstance(out, KVPlan) and out.ends.get_device() in here):  # its tensors were looked at when it was made
+            raise AssertionError("kv_plan: out is a KVPlan on the context's device")
+        if not (out.ends.numel() == 2 and out.starts.numel() == n + 1 and out.lens.numel() == n and out.slots.numel() == out.pos.numel() == out.seen.numel() == out.rows.numel() == capacity):
+            raise AssertionError("kv_plan: out was made for other sizes")
         rc = _lib.qeng_kv_plan(self.h, pool.h, n, lens.data_ptr(), add.data_ptr(), None if keep is None else keep.data_ptr(), table.data_ptr(), width,
                                ring.data_ptr(), ring.numel(), ends.data_ptr(), out.lens.data_ptr(), out.ends.data_ptr(), out.starts.data_ptr(),
                                out.slots.data_ptr(), out.pos.data_ptr(), out.seen.data_ptr(), out.rows.data_ptr(), capacity, _cur_stream())
@@ -435,12 +440,15 @@ class Context:
         (t, width), hd, i32, here = qkv.shape, pool.hd, torch.int32, self._here
         hq = width // hd - 2 * pool.kv_heads
         ld, one = qkv.stride()
-        assert qkv.is_cuda and qkv.get_device() in here and one == 1 and width % hd == 0
-        assert pos.is_cuda and slots.is_cuda and pos.get_device() in here and slots.get_device() in here and pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t
+        if not (qkv.is_cuda and qkv.get_device() in here and one == 1 and width % hd == 0):
+            raise AssertionError("rope_append: qkv is [T, heads * %d] on the context's device, rows of values side by side" % hd)
+        if not (pos.is_cuda and slots.is_cuda and pos.get_device() in here and slots.get_device() in here and pos.dtype is i32 and slots.dtype is i32 and pos.is_contiguous() and slots.is_contiguous() and pos.numel() == t and slots.numel() == t):
+            raise AssertionError("rope_append: pos and slots are contiguous int32 tensors [T] of the context's device")
         if out is None:
             out = qkv.new_empty((t, hq, hd), dtype=torch.float16)
         ldq, per_head, per_dim = out.stride()
-        assert out.is_cuda and out.get_device() in here and out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd
+        if not (out.is_cuda and out.get_device() in here and out.dtype is torch.float16 and out.shape == (t, hq, hd) and per_dim == 1 and per_head == hd):
+            raise AssertionError("rope_append: out is a float16 tensor [T, Hq, %d] of the context's device, heads side by side" % hd)
         rc = _lib.qeng_rope_append(self.h, pool.h, qkv.data_ptr(), _dtype(qkv), t, ld if t > 1 else width, hq,
                                    None if q_gain is None else _gain(q_gain, here), None if k_gain is None else _gain(k_gain, here), eps, pos.data_ptr(),
                                    slots.data_ptr(), base, out.data_ptr(), ldq if t > 1 else hq * hd, _cur_stream())
@@ -456,15 +464,19 @@ class Context:
         import torch
         (t, hq, hd), i32, here = q.shape, torch.int32, self._here
         ldq, per_head, per_dim = q.stride()
-        assert q.is_cuda and q.get_device() in here and q.dtype is torch.float16 and per_dim == 1 and per_head == hd == pool.hd
+        if not (q.is_cuda and q.get_device() in here and q.dtype is torch.float16 and per_dim == 1 and per_head == hd == pool.hd):
+            raise AssertionError("attn_shared: q is a float16 tensor [T, Hq, %d] of the context's device, heads side by side" % pool.hd)
         for x in (table, lens, group_first, group_pages) if rows is None else (table, lens, group_first, group_pages, rows):
-            assert x.is_cuda and x.get_device() in here and x.dtype is i32 and x.is_contiguous()
+            if not (x.is_cuda and x.get_device() in here and x.dtype is i32 and x.is_contiguous()):
+                raise AssertionError("attn_shared: table, lens, groups and rows are contiguous int32 tensors of the context's device")
         (table_rows, width), g = table.shape, group_pages.numel()
-        assert lens.numel() == t and group_first.numel() == g + 1 and (rows is None or rows.numel() == t)
+        if not (lens.numel() == t and group_first.numel() == g + 1 and (rows is None or rows.numel() == t)):
+            raise AssertionError("attn_shared: lens, rows or groups are too many or too few")
         if out is None:
             out = q.new_empty((t, hq, hd), dtype=dtype or torch.float32)
         ldo, per_head, per_dim = out.stride()
-        assert out.is_cuda and out.get_device() in here and out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd
+        if not (out.is_cuda and out.get_device() in here and out.shape == q.shape and (dtype is None or dtype is out.dtype) and per_dim == 1 and per_head == hd):
+            raise AssertionError("attn_shared: out is a tensor like q of the context's device, of the type asked for, heads side by side")
         rc = _lib.qeng_attn_shared(self.h, pool.h, q.data_ptr(), ldq if t > 1 else hq * hd, table.data_ptr(), width, table_rows,
                                    None if rows is None else rows.data_ptr(), lens.data_ptr(), t, hq, group_first.data_ptr(), group_pages.data_ptr(), g,
                                    float(hd) ** -0.5 if scale is None else scale, softcap, window, out.data_ptr(), _dtype(out), ldo if t > 1 else hq * hd,
@@ -490,7 +502,8 @@ def _dtype(t):
 
 def _gain(t, here):
     import torch
-    assert t.is_cuda and t.get_device() in here and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == 128
+    if not (t.is_cuda and t.get_device() in here and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == 128):
+        raise AssertionError("a gain is 128 contiguous float32 numbers on the context's device")
     return t.data_ptr()
 
 
@@ -520,7 +533,8 @@ class KVPlan(_PlanFields):
     def _checked(self):
         import torch
         for t in self:
-            assert t.is_cuda and t.get_device() == self.ends.get_device() and t.is_contiguous() and t.dtype is (torch.int64 if t is self.ends else torch.int32)
+            if not (t.is_cuda and t.get_device() == self.ends.get_device() and t.is_contiguous() and t.dtype is (torch.int64 if t is self.ends else torch.int32)):
+                raise AssertionError("KVPlan: contiguous tensors of one device, int32 but for ends (int64)")
         return self
 
 
