@@ -458,7 +458,8 @@ class Context:
 
     def attn_shared(self, pool, q, table, lens, group_first, group_pages, rows=None, scale=None, softcap=0.0, window=0, out=None, dtype=None):
         """Attention of rows q [T, Hq, 128] (float16) over lens[t] tokens of table row rows[t] (None: t), where the rows
-        group_first[g] .. group_first[g + 1] - 1 share their first group_pages[g] pages; see qeng_attn_shared.  The result is `out`, or new, of
+        group_first[g] .. group_first[g + 1] - 1 share their first group_pages[g] pages; see qeng_attn_shared (few rows are faster in
+        attn_decode).  The result is `out`, or new, of
         `dtype` (float32, float16 or bfloat16; None: float32); rows in no group, or of table row -1, are left alone (those of a new result
         are then not initialised)."""
         import torch

@@ -280,7 +280,7 @@ int32_t qeng_attn_decode_noalloc(qeng_ctx* ctx, const qeng_kv_pool* pool, const 
  *    makes no sense, gets nothing by itself (status 2).  New pages are written to the table.
  *  - a request that ends gives its pages back, but for the first keep[r] (keep may be NULL: none), which it shares with others.
  *    Pages given back are taken by later calls at the earliest.  Its length becomes 0, its row stays as it is.
- *  - starts[R + 1]: the first token of every request, and their number; per token up to `capacity`: slots (16 * page + place in the
+ *  - starts[R + 1]: the first token of every request, and their number (up to 1024 requests they will do as groups of qeng_attn_shared); per token up to `capacity`: slots (16 * page + place in the
  *    page), pos (its position), seen (pos + 1: the keys it attends), rows (its request).  Entries behind the last token are -1, 0, 0, -1.
  *  - lens_out, ends_out: lengths and counters afterwards.  They may be lens and ends themselves.
  * A page id outside the pool is reported (status 1): the slots in such a page are -1, and one that is given back goes into the ring as it
@@ -300,15 +300,20 @@ int32_t qeng_rope_append(qeng_ctx* ctx, qeng_kv_pool* pool, const void* qkv, int
                          const int32_t* slots, float base, uint16_t* q_f16, int64_t ldq, void* stream);
 /* out[t] = softmax(q[t] K^T * scale) V of every query head over the first lens[t] tokens of row rows[t] of page_table, for T rows
  * in G groups.  Group g is rows group_first[g] .. group_first[g + 1] - 1 (group_first ascends, G + 1 entries); their table rows begin
- * with the same group_pages[g] pages, which are read once for all of them (as the first row of the group lists them).  So a batch
+ * with the same group_pages[g] pages, which are read once for all of them (as any row of the group lists them).  So a batch
  * behind one prompt is a group whose pages are the prompt's, a prompt's own tokens are a group that shares all its pages (rows[t] the
- * request, lens[t] = position + 1: what qeng_kv_plan writes), and a row without company is a group of one with no page shared.
+ * request, lens[t] = position + 1: what qeng_kv_plan writes), and rows without company are, side by side, one group with no page shared
+ * (a group for each of them will do up to 1024).
+ * For few rows qeng_attn_decode is faster, which reads every row's pages in one kernel: up to 32 rows behind 1024 tokens, 16 behind
+ * 4096, 8 behind 16384 (32 query and 8 kv heads; 4 rows behind 512 tokens take 9 us there and 28 here).
  *  - q_f16[t] and out[t] (f32, f16 or bf16) are [Hq][128], ldq and ldo values from row to row.  rows may be NULL: row t has table
- *    row t.  A row in no group, or with rows[t] < 0, is left alone; one that attends nothing (lens[t] <= 0) gives zeros.
+ *    row t.  A row in no group, or with rows[t] < 0, is left alone; one that attends nothing (lens[t] <= 0) gives zeros; a length beyond
+ *    the table's row counts as far as that goes.
  *  - softcap and window as in qeng_attn_decode_ex: a row attends its last `window` tokens.  softcap is at most 1e30, and scale / softcap
  *    10^38 (QENG_ERR_ARG).
- *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of infinity or NaN, makes the
- *    results of the rows that attend it infinite or NaN, and of no other row.
+ *  - f32 results keep the weights to 22 bits, 16-bit results to 11.  A value of infinity, and a score of plus infinity or NaN, makes the
+ *    results of the rows that attend it infinite or NaN, and of no other row; a key whose score is minus infinity weighs nothing (a row
+ *    that attends no other is NaN).  softcap brings infinite scores to plus or minus softcap.
  * hd = 128, Hq / kv_heads <= 8, scale >= 0, G <= 1024, T * Hq <= 2^21, G + T * Hq / kv_heads / 240 < 4096.  Bounds of groups that do
  * not ascend, and rows outside the table, are reported (status 6; with such bounds nothing is written).  A page id outside the pool is
  * reported (status 1): no page is read in its place, and what the rows that attend it get means nothing.  Needs working memory of the

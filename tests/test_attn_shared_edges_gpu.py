@@ -70,3 +70,25 @@ def test_caps_that_leave_32_bits_are_refused(ctx):
     b.pool.free()
     check(ctx, [behind(3, [5])], 8, 2, softcap=1e30)
     check(ctx, [behind(3, [5])], 8, 2, softcap=1e-30, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("softcap", [30.0, 1000.0])
+def test_a_cap_brings_infinite_scores_to_itself(ctx, softcap, dtype):
+    """Among shared pages and a row's own; NaN stays NaN."""
+    import torch
+    for shared in (0, 6):
+        b = Batch(ctx, [(6, [96, 80, 17, 3])], 4, 1, junk=0.0)
+        b.table_np[:] = b.table_np[0]
+        b.table, b.shared = _ints(b.table_np), [shared]
+        data = b.pool.tensor()
+        b.q[:, :, 0] = 1.0
+        at = [int(b.table_np[0, k]) for k in (1, 4)]
+        data[at[0], 0, 0, 5, 0], data[at[1], 0, 0, 9, 0] = math.inf, -math.inf
+        a, kw = b.args()
+        got = ctx.attn_shared(*a, **kw, softcap=softcap, dtype=getattr(torch, dtype))
+        assert_near(got, *b.exact(softcap=softcap))
+        data[at[0], 0, 0, 5, 0] = math.nan
+        got = ctx.attn_shared(*a, **kw, softcap=softcap, dtype=getattr(torch, dtype))
+        assert bool(torch.isnan(got[:2]).all()) and bool(torch.isfinite(got[3]).all())
+        b.pool.free()
