@@ -254,9 +254,12 @@ __device__ __forceinline__ void add_pieces(int lane, int c0, int c1, const float
 //
 // K and V tiles: [2 halves of 64 dims][128 keys][128 bytes], 128-byte swizzled; K is a K-major operand of 128 columns, V an MN-major one.
 //
-// Bound by the chain of a tile: 128 keys of both tiles take 3550 cycles, of which the MMAs need 2048 and the powers of two as many (16 a
-// cycle and SM); a tile's softmax takes 2150 of them and then waits 1400 for its values and the next scores.  256 rows behind 16384 tokens,
-// 32 query and 8 kv heads: 78 us (69 GFLOP, 0.53 of the measured rate; the tensor pipe is busy for 44 % of the cycles).  What did not
+// Bound by the chain of a tile: 128 keys of both tiles take 3650 cycles, of which the MMAs need 2048 and the powers of two as many (16 a
+// cycle and SM); a tile's softmax takes 2600 of them and then waits 1050 for its values and the next scores.  With two terms 7200 cycles.
+// 256 rows behind 16384 tokens, 32 query and 8 kv heads: 78 us (69 GFLOP, 0.53 of the measured rate; the tensor pipe is busy for 44 % of
+// the cycles), of which 3 us are the look at all rows in front.  Seven prompts of 7551 rows: 365 us.  A CTA's blocks are as many as another's,
+// but from one (double tile, kv head) to the next takes 12000 cycles, and a CTA has 4 to 25 of them there: CTAs end between 40 and 372 us,
+// half of them before 266, and the look at all rows takes 13 us (39 in the CTA that counts units).  What did not
 // help, each measured against the kernel of its time: eight softmax warps a tile (96 registers and spills: 110 us, 92 without), a warp of
 // its own for each tile's MMAs (the tiles fall into step and wait together: 4900 cycles for 128 keys), scores of 64 keys in two buffers
 // (an MMA of 64 columns takes 74 cycles: 107 us, 92 without), part of the powers as polynomials on the FMA pipe (a call 133 us, 129
@@ -929,7 +932,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attn_tile_kernel(const qeng_s
 // ---- a row's own pages ------------------------------------------------------------------------------------------------------
 // Every warp has pages of its own, of one or several (row, kv head), and keeps two on their way.  HBM-bound where there are many pages:
 // 256 rows of 1 to 256 tokens (134 MB) take 29 us (4.6 TB/s), 64 of 1 to 1024 27 us; below that a start and an end, 4 to 5 us, and 1 us
-// a page.  With a (row, kv head) for the four warps of a CTA, merged in shared memory, these took 57 and 48 us.  The query heads of the
+// a page.  Three CTAs fit on an SM up to about 840 groups, above that two, but the work is cut for three: 1000 rows of 1024 tokens take
+// 718 us in as many groups, 661 in one.  With a (row, kv head) for the four warps of a CTA, merged in shared memory, these took 57 and 48 us.  The query heads of the
 // kv head are the eight columns of every MMA, S^T = K Q^T and O^T = V^T P^T; P in two f16 terms.
 __global__ void __launch_bounds__(kThreads, 3) attn_own_kernel(const qeng_shared_attn p, const __grid_constant__ CUtensorMap kvmap) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
